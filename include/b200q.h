@@ -297,11 +297,89 @@ int b200q_gemm_swiglu_cast(const void* a, int lda, const void* bq, const void* s
                            int act_dtype, int cast_group, int use_clamp, float clamp_value, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* ---- 8-bit integers on both sides ----------------------------------------------------------------------
+ * The compute-bound route beside b200q_gemm (no counterpart in the reference): activations cast per token,
+ * weights per channel, exact int32 sums.
+ *
+ * b200q_per_token_cast_int: per row of x[tokens, hidden] (fp16 or bf16, row stride ldx elements, hidden a multiple of 8)
+ * with m = max |x|: out = rint(x * (127 / m)) as int8 (row stride ldo), out_sf = m / 127 (fp32 [tokens]); quotients and
+ * product are rounded to fp32.  A row with m < 2^-100 counts as zero (codes 0, scale 1).  A row with a NaN or an
+ * infinity has it as its scale: products with it are NaN.  (Weights [N, K] are cast by the same call, a row a channel.)
+ *
+ * b200q_igemm: C[M, N] = A x B^T * a_sf[m] * b_sf[n] + bias[n] with int8 A[M, K] (row stride lda) and B[N, K] (row
+ * stride ldb), fp32 scales, C and bias (NULL: none) of act_dtype.  K and N are multiples of 16, K <= 131056; lda and ldb
+ * multiples of 16, ldc of 8; a, b, c, b_sf and bias aligned to 16 bytes.  The sums are int32 and exact; the scales are
+ * applied in fp32, in the order written.
+ *
+ * b200q_igemm_swiglu: B[2 N, K] holds the gate rows first; with g, u the two scaled products of a column,
+ * C = g / (1 + exp(-g)) * u; with use_clamp g is clamped from above and u on both sides to clamp_value, as in
+ * b200q_swiglu_per_token_cast.  One kernel: neither product is written.
+ *
+ * b200q_igemm_plan names the kernel these calls take; b200q_igemm_planned runs an edited plan.  `workspace` holds the
+ * status header (256 bytes, zeroed once, as for the other calls of the stream).  The kernels set up under the end of
+ * the stream's previous kernel, and read nothing before that has ended. */
+typedef struct b200q_igemm_plan {
+  int32_t kernel;  /* 1: pairs of CTAs, 256 rows x 256 product columns a tile; 2: B streamed once (M <= 256) */
+  int32_t rows;    /* kernel 2: M rounded up to 16 (output only) */
+  int32_t cluster; /* kernel 2: CTAs that share a column tile's K, 1 .. 8 */
+  int32_t stages;  /* kernel 2: ring slots of 128 bytes of K, 2 .. 12 */
+  int32_t ctas;    /* kernel 1: CTAs, even; kernel 2: output only */
+} b200q_igemm_plan_t;
+int b200q_per_token_cast_int(const void* x, int ldx, void* out, int ldo, float* out_sf, int tokens, int hidden,
+                             int act_dtype, void* stream);
+int b200q_igemm(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, const void* bias,
+                void* c, int ldc, int M, int N, int K, int act_dtype, void* workspace, size_t workspace_bytes,
+                void* stream);
+int b200q_igemm_swiglu(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, void* c,
+                       int ldc, int M, int N, int K, int act_dtype, int use_clamp, float clamp_value, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int b200q_igemm_plan(int M, int N, int K, int gated, b200q_igemm_plan_t* plan);
+int b200q_igemm_planned(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf,
+                        const void* bias, void* c, int ldc, int M, int N, int K, int act_dtype, int gated, int use_clamp,
+                        float clamp_value, void* workspace, size_t workspace_bytes, void* stream,
+                        const b200q_igemm_plan_t* plan);
+
+/* ---- the norms before and after a block, with its gate and residual scale --------------------------------
+ * What stands between two blocks of a decoder, in one kernel (no counterpart in the reference).  For each row t:
+ *
+ *   n  = block * rsqrt(mean(block^2) + eps) * post_weight     (post_weight NULL: n = block)
+ *   r' = residual_scale * residual + gate * n                 (residual NULL: zero; gate NULL: one)
+ *   x  = r' * rsqrt(mean(r'^2) + eps) * weight
+ *
+ * block, weight, post_weight and gate are of act_dtype; residual and r' too, or fp32 (residual_f32).  `gates` rows of gate
+ * serve tokens / gates consecutive rows each (1: a gate per channel).  hidden is a multiple of 8, at most 16384; all pointers
+ * are aligned to 16 bytes and all row strides (elements) multiples of 8.  fp32 throughout: x comes from the unrounded r'.
+ *
+ * b200q_block_norm writes r' to new_residual (row stride ldn; it may be the residual itself) and either x (row stride ldx) or,
+ * with x NULL, x_int and x_sf: the per-token int8 cast of the rounded x, the codes of b200q_per_token_cast_int.
+ *
+ * b200q_block_norm_backward: from grad_x (act_dtype) and grad_new (of r', its type; NULL: zero) the gradients of block
+ * (act_dtype), residual (its type; NULL: not wanted), and in fp32 of weight [hidden], post_weight [hidden] and gate
+ * [gates, hidden] (given exactly where the operand is).  What the forward pass computed is computed again from its inputs.
+ * `scratch`: b200q_block_norm_scratch_bytes(...) bytes of this call's own, need not be cleared.  The same inputs give the
+ * same bits. */
+typedef struct b200q_block_norm {
+  const void *block, *residual, *weight, *post_weight, *gate;
+  int64_t ldb, ldr, ldg;  /* row strides of block, residual, gate */
+  int32_t tokens, hidden;
+  int32_t gates;          /* rows of gate, 0 without */
+  int32_t act_dtype, residual_f32;
+  float residual_scale, eps;
+} b200q_block_norm_t;
+int b200q_block_norm(const b200q_block_norm_t* args, void* x, long long ldx, void* x_int, float* x_sf, void* new_residual,
+                     long long ldn, void* stream);
+size_t b200q_block_norm_scratch_bytes(int tokens, int hidden, int gates);
+int b200q_block_norm_backward(const b200q_block_norm_t* args, const void* grad_x, long long lddx, const void* grad_new,
+                              long long lddn, void* grad_block, long long lddb, void* grad_residual, long long lddr,
+                              float* grad_weight, float* grad_post, float* grad_gate, void* scratch, size_t scratch_bytes,
+                              void* stream);
+
 /* Reads the device status header of a workspace (synchronises `stream`): status[0] is 0 or
  * B200Q_ERR_DEVICE_TIMEOUT, status[1..3] say which wait gave up (1: 2 = tcgen05 prefill pipeline,
  * 3 = stream kernel's weight ring, 5 = wait for a peer's columns, 6 = tcgen05 small-batch pipeline,
  * 7 / 8 = gather push / collect, 9 = wait for the CTAs that fetch host activations, 10 = exact
- * small-batch kernel's pipeline, 11 = a wait of the kernel that keeps the activations in registers; 2: CTA; 3: warp or thread).  Clears the header.  A launch that gave up may leave partial sums
+ * small-batch kernel's pipeline, 11 = a wait of the kernel that keeps the activations in registers, 12 = pair kernel of
+ * the 8-bit products, 13 = their stream kernel; 2: CTA; 3: warp or thread).  Clears the header.  A launch that gave up may leave partial sums
  * behind: zero the workspace before it is used again.  workspace == NULL names the built-in
  * scratch of b200q_gemm_static_ws, which this call then puts back to zero itself. */
 int b200q_device_status(void* workspace, int32_t status[4], void* stream);

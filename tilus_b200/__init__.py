@@ -1,5 +1,8 @@
 """B200-native weight-only quantized matmul (drop-in for the reference's
-examples/quantization/matmul_a16wx.py operator surface)."""
+examples/quantization/matmul_a16wx.py operator surface), and what a decoder needs around it."""
 from .dtypes import *  # noqa: F401,F403
+from .int8 import Int8Linear  # noqa: E402,F401
 from .linear import QuantizedLinear  # noqa: E402,F401
-from .ops import dequantize, quantized_matmul  # noqa: E402,F401
+from .norm import BlockNorm  # noqa: E402,F401
+from .ops import (block_norm, block_norm_backward, block_norm_cast_int8, dequantize, int8_gate_up,  # noqa: E402,F401
+                  int8_matmul, per_token_cast_int8, quantized_matmul)

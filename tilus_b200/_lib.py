@@ -63,8 +63,25 @@ class Plan(ctypes.Structure):
         return {n: int(getattr(self, n)) for n, _ in self._fields_}
 
 
+class IgemmPlan(ctypes.Structure):
+    """b200q_igemm_plan_t of include/b200q.h."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "rows", "cluster", "stages", "ctas")]
+
+    def as_dict(self):
+        return {n: int(getattr(self, n)) for n, _ in self._fields_}
+
+
+class BlockNorm(ctypes.Structure):
+    """b200q_block_norm_t of include/b200q.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("block", "residual", "weight", "post_weight", "gate")]
+                + [(n, ctypes.c_int64) for n in ("ldb", "ldr", "ldg")]
+                + [(n, ctypes.c_int32) for n in ("tokens", "hidden", "gates", "act_dtype", "residual_f32")]
+                + [(n, ctypes.c_float) for n in ("residual_scale", "eps")])
+
+
 # every symbol include/b200q.h declares: name -> (restype, argtypes)
 _vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_ll, _f = ctypes.c_longlong, ctypes.c_float
 SYMBOLS = {
     "b200q_version": (_i, []),
     "b200q_layout_version": (_i, []),
@@ -94,6 +111,16 @@ SYMBOLS = {
     "b200q_swiglu_per_token_cast": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, ctypes.c_float, _vp]),
     "b200q_gemm_swiglu_cast": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i,
                                     ctypes.c_float, _vp, _sz, _vp]),
+    "b200q_per_token_cast_int": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _vp]),
+    "b200q_igemm": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "b200q_igemm_swiglu": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp]),
+    "b200q_igemm_plan": (_i, [_i, _i, _i, _i, ctypes.POINTER(IgemmPlan)]),
+    "b200q_igemm_planned": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp,
+                                 ctypes.POINTER(IgemmPlan)]),
+    "b200q_block_norm": (_i, [ctypes.POINTER(BlockNorm), _vp, _ll, _vp, _vp, _vp, _ll, _vp]),
+    "b200q_block_norm_scratch_bytes": (_sz, [_i, _i, _i]),
+    "b200q_block_norm_backward": (_i, [ctypes.POINTER(BlockNorm), _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp,
+                                       _sz, _vp]),
     "b200q_device_status": (_i, [_vp, ctypes.POINTER(ctypes.c_int32 * 4), _vp]),
 }
 
@@ -140,6 +167,9 @@ def native():
         addresses = [ctypes.cast(getattr(lib, "b200q_" + name), ctypes.c_void_p).value
                      for name in ("gemm", "gemm_host", "gemm_swiglu_cast", "workspace_bytes")]
         ext.bind(*addresses, check, unsupported)
+        ext.bind_int8(*(ctypes.cast(getattr(lib, "b200q_" + name), ctypes.c_void_p).value
+                        for name in ("per_token_cast_int", "igemm", "igemm_swiglu", "block_norm",
+                                     "block_norm_scratch_bytes", "block_norm_backward")))
         _native = ext
     return _native
 

@@ -57,6 +57,9 @@ def _jobs():
     jobs.append(("cast_kernel.cu", "cast.o", []))
     jobs.append(("gather_kernel.cu", "gather.o", []))
     jobs.append(("fetch_kernel.cu", "fetch.o", []))
+    jobs.append(("int8_kernel.cu", "int8.o", []))
+    jobs.append(("norm_kernel.cu", "norm.o", []))
+    jobs.append(("int8_api.cu", "int8_api.o", []))
     jobs.append(("api.cu", "api.o", [f"-DB200Q_NPARTS={NPARTS}"]))
     return jobs
 

@@ -9,6 +9,7 @@
 
 #include "../../include/b200q.h"
 #include "common.cuh"
+#include "int8.cuh"
 
 #ifndef B200Q_NPARTS
 #define B200Q_NPARTS 8
@@ -55,6 +56,10 @@ int umma_smem_bytes(int tm, int bits, int a_stages, int rpg);
 int umma_a_stages(int tm, int bits, int max_smem, int rpg);
 
 static thread_local int g_last_cuda_error = 0;
+int cuda_failed(int code) {
+  g_last_cuda_error = code;
+  return ST_CUDA;
+}
 
 static cudaError_t stream_launch(int var, const StreamParams& p, int mt, int smem, cudaStream_t s) {
   switch (var % B200Q_NPARTS) {
@@ -122,10 +127,7 @@ static cudaError_t umma_launch(int var, const UmmaParams& p, const void* tmap, i
 }
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point lookup (no link to libcuda)
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_tiled_fn() {
+EncodeTiledFn encode_tiled_fn() {
   static EncodeTiledFn fn = nullptr;
   if (!fn) {
     void* ptr = nullptr;
@@ -154,11 +156,7 @@ static int variant_of(int wtype, int zero_point) {
   return -1;
 }
 
-struct DeviceInfo {
-  int sm_count = 0;
-  int max_smem = 0;
-};
-static DeviceInfo device_info() {
+DeviceInfo device_info() {
   static DeviceInfo cache[16];
   int dev = 0;
   cudaGetDevice(&dev);

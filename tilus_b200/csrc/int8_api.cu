@@ -1,0 +1,298 @@
+// C ABI of the 8-bit integer products, the per-token int8 cast and the block norms: argument checks, kernel choice, launches.
+#include <cmath>
+
+#include "../../include/b200q.h"
+#include "int8.cuh"
+#include "norm.cuh"
+
+namespace b200q {
+
+static bool misaligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
+static bool known_act(int act) { return act == B200Q_F16 || act == B200Q_BF16; }
+
+// ---- products -----------------------------------------------------------------------------------------------
+// int32 sums are exact up to this K: 128 * 128 * K < 2^31
+static const int kInt8MaxK = 131056;
+static const int kStreamRows = 256;
+
+static int check_igemm(int M, int N, int K) {
+  if (M < 1 || N < 1 || K < 1) return ST_INVALID_ARG;
+  if (N % 16 != 0 || K % 16 != 0 || K > kInt8MaxK) return ST_UNSUPPORTED;
+  return ST_OK;
+}
+static int igemm_kblocks(int K) { return (K + 127) / 128; }
+
+static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) {
+  const DeviceInfo di = device_info();
+  *pl = b200q_igemm_plan_t();
+  if (M > kStreamRows) {
+    pl->kernel = 1;
+    pl->rows = 256;
+    pl->cluster = 2;
+    const int tiles = ((M + 255) / 256) * ((N + (gated ? 127 : 255)) / (gated ? 128 : 256));
+    pl->ctas = 2 * (tiles < di.sm_count / 2 ? tiles : di.sm_count / 2);
+    pl->stages = 6;
+    return;
+  }
+  pl->kernel = 2;
+  pl->rows = (M + 15) / 16 * 16;
+  const int cols = gated ? 64 : 128, tiles = (N + cols - 1) / cols;
+  const int per_sm = pl->rows <= 64 ? 2 : 1;
+  int s = per_sm * di.sm_count / tiles;
+  const int most = (igemm_kblocks(K) + 3) / 4;
+  if (s > most) s = most;
+  pl->cluster = s < 1 ? 1 : s > 8 ? 8 : s;
+  pl->ctas = tiles * pl->cluster;
+  const int budget = per_sm == 2 ? 113 * 1024 : di.max_smem;
+  pl->stages = 12;
+  while (pl->stages > 2 && int8_stream_smem_bytes(pl->rows, pl->stages) > budget) --pl->stages;
+}
+
+// 2-D map of 8-bit rows, a box of 128 bytes x `rows`
+static int encode_rows(EncodeTiledFn enc, CUtensorMap* map, const void* base, int K, long long rows, long long ld, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows}, steps[2] = {1u, 1u};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, steps,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? ST_OK : cuda_failed((int)r);
+}
+
+static int run_igemm(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, const void* bias, void* c,
+                     int ldc, int M, int N, int K, int act, bool gated, int use_clamp, float clamp, void* workspace, size_t ws_bytes,
+                     cudaStream_t stream, const b200q_igemm_plan_t& pl) {
+  if (!known_act(act)) return ST_UNSUPPORTED;
+  int st = check_igemm(M, N, K);
+  if (st != ST_OK) return st;
+  if (!a || !b || !a_sf || !b_sf || !c) return ST_INVALID_ARG;
+  if (lda < K || ldb < K || ldc < N || lda % 16 != 0 || ldb % 16 != 0 || ldc % 8 != 0) return ST_INVALID_ARG;
+  if (misaligned(a, 16) || misaligned(b, 16) || misaligned(c, 16) || misaligned(a_sf, 4) || misaligned(b_sf, 16) || misaligned(bias, 16))
+    return ST_INVALID_ARG;
+  if (use_clamp && std::isnan(clamp)) return ST_INVALID_ARG;
+  if (!workspace || ws_bytes < WS_HEADER_BYTES || misaligned(workspace, 256)) return ST_WORKSPACE;
+  const EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return cuda_failed((int)cudaErrorNotSupported);
+  Int8Params p = {};
+  p.a_sf = a_sf; p.b_sf = b_sf;
+  p.bias = static_cast<const unsigned short*>(bias);
+  p.c = static_cast<unsigned short*>(c);
+  p.status = static_cast<int*>(workspace);
+  p.M = M; p.N = N; p.K = K; p.ldc = ldc;
+  p.kblocks = igemm_kblocks(K);
+  p.act = act;
+  p.use_clamp = use_clamp ? 1 : 0;
+  p.clamp = clamp;
+  const long long b_rows = gated ? 2ll * N : N;
+  CUtensorMap ta, tb, tc;
+  cudaError_t e;
+  if (pl.kernel == 1) {
+    st = encode_rows(enc, &ta, a, K, M, lda, 128);
+    if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, 128);
+    if (st != ST_OK) return st;
+    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+    const cuuint64_t strides[1] = {(cuuint64_t)ldc * 2};
+    const cuuint32_t box[2] = {64u, 128u}, steps[2] = {1u, 1u};
+    const CUresult r = enc(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, c, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return cuda_failed((int)r);
+    p.m_tiles = (int)(((long long)M + 255) / 256);
+    p.n_tiles = (N + (gated ? 127 : 255)) / (gated ? 128 : 256);
+    if ((long long)p.m_tiles * p.n_tiles > 0x7fffffffll) return ST_UNSUPPORTED;
+    p.tiles = p.m_tiles * p.n_tiles;
+    // rows of A that stay in the L2 cache while the columns of B stream past them: about 32 MB
+    const long long fit = (32ll << 20) / (256ll * K);
+    p.m_group = (int)(fit < 1 ? 1 : fit > p.m_tiles ? p.m_tiles : fit);
+    e = int8_pair_launch(p, gated, ta, tb, tc, pl.ctas, stream);
+  } else {
+    st = encode_rows(enc, &ta, a, K, M, lda, pl.rows);
+    if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, gated ? 64 : 128);
+    if (st != ST_OK) return st;
+    p.rows = pl.rows; p.cluster = pl.cluster; p.stages = pl.stages;
+    p.tiles = pl.ctas / pl.cluster;
+    e = int8_stream_launch(p, gated, ta, tb, stream);
+  }
+  return e == cudaSuccess ? ST_OK : cuda_failed((int)e);
+}
+
+// Whether a (possibly edited) plan can be run: what its kernel needs of its fields.
+static bool igemm_plan_ok(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) {
+  const DeviceInfo di = device_info();
+  if (pl->kernel == 1) {
+    if (pl->ctas < 2 || pl->ctas % 2 != 0 || pl->ctas > di.sm_count) return false;
+    return int8_pair_smem_bytes() <= di.max_smem;
+  }
+  if (pl->kernel != 2 || M > kStreamRows) return false;
+  pl->rows = (M + 15) / 16 * 16;
+  const int cols = gated ? 64 : 128;
+  if (pl->cluster < 1 || pl->cluster > 8 || pl->cluster > igemm_kblocks(K)) return false;
+  pl->ctas = (N + cols - 1) / cols * pl->cluster;
+  return pl->stages >= 2 && pl->stages <= 12 && int8_stream_smem_bytes(pl->rows, pl->stages) <= di.max_smem;
+}
+
+// ---- row-wise kernels -------------------------------------------------------------------------------------
+static const int kNormMaxD = 16384;
+
+// CTAs of the gradient's launch: whole rounds of the GPU, split evenly over the gates
+static void norm_backward_grid(int T, int D, int gates, int* grid, int* per_gate) {
+  const int sms = device_info().sm_count, nvec = D / 8;
+  const int most = sms * (nvec <= 128 ? 4 : nvec <= 256 ? 2 : 1);
+  const int tokens = T / gates;
+  if (gates >= most) {
+    *per_gate = 1;
+    *grid = most;
+  } else {
+    *per_gate = most / gates < tokens ? most / gates : tokens;
+    *grid = gates * *per_gate;
+  }
+}
+
+}  // namespace b200q
+
+using namespace b200q;
+
+extern "C" {
+
+int b200q_igemm_plan(int M, int N, int K, int gated, b200q_igemm_plan_t* plan) {
+  if (!plan) return ST_INVALID_ARG;
+  const int st = check_igemm(M, N, K);
+  if (st == ST_OK) plan_igemm(M, N, K, gated != 0, plan);
+  return st;
+}
+
+int b200q_igemm(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, const void* bias, void* c, int ldc,
+                int M, int N, int K, int act_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_igemm(M, N, K);
+  if (st != ST_OK) return st;
+  b200q_igemm_plan_t pl;
+  plan_igemm(M, N, K, false, &pl);
+  return run_igemm(a, lda, b, ldb, a_sf, b_sf, bias, c, ldc, M, N, K, act_dtype, false, 0, 0.f, workspace, workspace_bytes,
+                   static_cast<cudaStream_t>(stream), pl);
+}
+
+int b200q_igemm_swiglu(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, void* c, int ldc, int M,
+                       int N, int K, int act_dtype, int use_clamp, float clamp_value, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  int st = check_igemm(M, N, K);
+  if (st != ST_OK) return st;
+  if (N > 0x7fffffff / 2) return ST_UNSUPPORTED;
+  b200q_igemm_plan_t pl;
+  plan_igemm(M, N, K, true, &pl);
+  return run_igemm(a, lda, b, ldb, a_sf, b_sf, nullptr, c, ldc, M, N, K, act_dtype, true, use_clamp, clamp_value, workspace,
+                   workspace_bytes, static_cast<cudaStream_t>(stream), pl);
+}
+
+int b200q_igemm_planned(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, const void* bias, void* c,
+                        int ldc, int M, int N, int K, int act_dtype, int gated, int use_clamp, float clamp_value, void* workspace,
+                        size_t workspace_bytes, void* stream, const b200q_igemm_plan_t* plan) {
+  int st = check_igemm(M, N, K);
+  if (st != ST_OK) return st;
+  if (!plan || (gated && (bias || N > 0x7fffffff / 2))) return ST_INVALID_ARG;
+  b200q_igemm_plan_t pl = *plan;
+  if (!igemm_plan_ok(M, N, K, gated != 0, &pl)) return ST_UNSUPPORTED;
+  return run_igemm(a, lda, b, ldb, a_sf, b_sf, bias, c, ldc, M, N, K, act_dtype, gated != 0, use_clamp, clamp_value, workspace,
+                   workspace_bytes, static_cast<cudaStream_t>(stream), pl);
+}
+
+int b200q_per_token_cast_int(const void* x, int ldx, void* out, int ldo, float* out_sf, int tokens, int hidden, int act_dtype,
+                             void* stream) {
+  if (!known_act(act_dtype)) return ST_UNSUPPORTED;
+  if (!x || !out || !out_sf || tokens < 1 || hidden < 1) return ST_INVALID_ARG;
+  if (hidden % 8 != 0) return ST_UNSUPPORTED;
+  if (ldx < hidden || ldo < hidden || ldx % 8 != 0 || ldo % 8 != 0) return ST_INVALID_ARG;
+  if (misaligned(x, 16) || misaligned(out, 8) || misaligned(out_sf, 4)) return ST_INVALID_ARG;
+  CastIntParams p;
+  p.x = static_cast<const unsigned short*>(x);
+  p.out = static_cast<signed char*>(out);
+  p.out_sf = out_sf;
+  p.T = tokens; p.D = hidden; p.ldx = ldx; p.ldo = ldo;
+  const cudaError_t e = cast_int_launch(p, act_dtype, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ST_OK : cuda_failed((int)e);
+}
+
+static int check_norm(const b200q_block_norm_t* a) {
+  if (!a) return ST_INVALID_ARG;
+  if (!known_act(a->act_dtype)) return ST_UNSUPPORTED;
+  if (!a->block || !a->weight || a->tokens < 1 || a->hidden < 1 || a->gates < 0) return ST_INVALID_ARG;
+  if ((a->gates == 0) != (a->gate == nullptr)) return ST_INVALID_ARG;
+  if (a->hidden % 8 != 0 || a->hidden > kNormMaxD) return ST_UNSUPPORTED;
+  if (a->gates > 0 && a->tokens % a->gates != 0) return ST_INVALID_ARG;
+  if (a->ldb < a->hidden || a->ldb % 8 != 0) return ST_INVALID_ARG;
+  if (a->residual && (a->ldr < a->hidden || a->ldr % 8 != 0)) return ST_INVALID_ARG;
+  if (a->gates > 1 && (a->ldg < a->hidden || a->ldg % 8 != 0)) return ST_INVALID_ARG;
+  if (misaligned(a->block, 16) || misaligned(a->residual, 16) || misaligned(a->weight, 16) || misaligned(a->post_weight, 16) ||
+      misaligned(a->gate, 16))
+    return ST_INVALID_ARG;
+  return ST_OK;
+}
+
+int b200q_block_norm(const b200q_block_norm_t* a, void* x, long long ldx, void* x_int, float* x_sf, void* new_residual, long long ldn,
+                     void* stream) {
+  const int st = check_norm(a);
+  if (st != ST_OK) return st;
+  if ((x == nullptr) == (x_int == nullptr) || (x_int && !x_sf) || !new_residual) return ST_INVALID_ARG;
+  if (ldx < a->hidden || ldx % 8 != 0 || ldn < a->hidden || ldn % 8 != 0) return ST_INVALID_ARG;
+  if (misaligned(x, 16) || misaligned(x_int, 8) || misaligned(x_sf, 4) || misaligned(new_residual, 16)) return ST_INVALID_ARG;
+  NormParams p = {};
+  p.block = static_cast<const unsigned short*>(a->block);
+  p.weight = static_cast<const unsigned short*>(a->weight);
+  p.post = static_cast<const unsigned short*>(a->post_weight);
+  p.gate = static_cast<const unsigned short*>(a->gate);
+  p.residual = a->residual;
+  p.x = static_cast<unsigned short*>(x);
+  p.x_int = static_cast<signed char*>(x_int);
+  p.x_sf = x_sf;
+  p.new_residual = new_residual;
+  p.T = a->tokens; p.D = a->hidden;
+  p.tokens_per_gate = a->gates > 0 ? a->tokens / a->gates : a->tokens;
+  p.ldb = a->ldb; p.ldr = a->ldr; p.ldg = a->ldg; p.ldx = ldx; p.ldn = ldn;
+  p.scale = a->residual_scale; p.eps = a->eps;
+  const cudaError_t e = norm_launch(p, a->act_dtype, a->residual_f32 != 0, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ST_OK : cuda_failed((int)e);
+}
+
+size_t b200q_block_norm_scratch_bytes(int tokens, int hidden, int gates) {
+  if (tokens < 1 || hidden < 8 || hidden % 8 != 0 || hidden > kNormMaxD || gates < 0 || (gates > 0 && tokens % gates != 0)) return 0;
+  int grid, per_gate;
+  norm_backward_grid(tokens, hidden, gates > 0 ? gates : 1, &grid, &per_gate);
+  return (size_t)3 * grid * hidden * sizeof(float);
+}
+
+int b200q_block_norm_backward(const b200q_block_norm_t* a, const void* grad_x, long long lddx, const void* grad_new, long long lddn,
+                              void* grad_block, long long lddb, void* grad_residual, long long lddr, float* grad_weight,
+                              float* grad_post, float* grad_gate, void* scratch, size_t scratch_bytes, void* stream) {
+  const int st = check_norm(a);
+  if (st != ST_OK) return st;
+  if (!grad_x || !grad_block || !grad_weight || (grad_post == nullptr) != (a->post_weight == nullptr) ||
+      (grad_gate == nullptr) != (a->gate == nullptr) || (grad_residual && !a->residual))
+    return ST_INVALID_ARG;
+  if (lddx < a->hidden || lddx % 8 != 0 || lddb < a->hidden || lddb % 8 != 0) return ST_INVALID_ARG;
+  if ((grad_new && (lddn < a->hidden || lddn % 8 != 0)) || (grad_residual && (lddr < a->hidden || lddr % 8 != 0))) return ST_INVALID_ARG;
+  if (misaligned(grad_x, 16) || misaligned(grad_new, 16) || misaligned(grad_block, 16) || misaligned(grad_residual, 16) ||
+      misaligned(grad_weight, 16) || misaligned(grad_post, 16) || misaligned(grad_gate, 16))
+    return ST_INVALID_ARG;
+  if (!scratch || misaligned(scratch, 16) || scratch_bytes < b200q_block_norm_scratch_bytes(a->tokens, a->hidden, a->gates))
+    return ST_WORKSPACE;
+  NormBackwardParams p = {};
+  p.block = static_cast<const unsigned short*>(a->block);
+  p.weight = static_cast<const unsigned short*>(a->weight);
+  p.post = static_cast<const unsigned short*>(a->post_weight);
+  p.gate = static_cast<const unsigned short*>(a->gate);
+  p.grad_x = static_cast<const unsigned short*>(grad_x);
+  p.residual = a->residual; p.grad_new = grad_new;
+  p.grad_block = static_cast<unsigned short*>(grad_block);
+  p.grad_residual = grad_residual;
+  p.grad_weight = grad_weight; p.grad_post = grad_post; p.grad_gate = grad_gate;
+  p.partial = static_cast<float*>(scratch);
+  p.T = a->tokens; p.D = a->hidden;
+  p.gates = a->gates > 0 ? a->gates : 1;
+  p.tokens_per_gate = a->tokens / p.gates;
+  norm_backward_grid(p.T, p.D, p.gates, &p.grid, &p.ctas_per_gate);
+  p.ldb = a->ldb; p.ldr = a->ldr; p.ldg = a->ldg;
+  p.lddx = lddx; p.lddn = lddn; p.lddb = lddb; p.lddr = lddr;
+  p.scale = a->residual_scale; p.eps = a->eps;
+  const cudaError_t e = norm_backward_launch(p, a->act_dtype, a->residual_f32 != 0, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ST_OK : cuda_failed((int)e);
+}
+
+}  // extern "C"

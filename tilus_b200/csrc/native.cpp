@@ -1,4 +1,4 @@
-// Host path of QuantizedLinear as a CPython extension (tilus_b200._native): argument checks, output and
+// Host path of QuantizedLinear, and of the 8-bit integer operators and block norms, as a CPython extension (tilus_b200._native): argument checks, output and
 // workspace tensors, stream lookup and the call into libb200q, in one native function per call.
 //
 // A decode call occupies the GPU for 5..15 us, so a program that calls its layers one by one is bound by
@@ -369,6 +369,296 @@ PyObject* workspace(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- 8-bit integer operators and block norms ------------------------------------------------------------
+decltype(&b200q_per_token_cast_int) g_cast_int = nullptr;
+decltype(&b200q_igemm) g_igemm = nullptr;
+decltype(&b200q_igemm_swiglu) g_igemm_swiglu = nullptr;
+decltype(&b200q_block_norm) g_norm = nullptr;
+decltype(&b200q_block_norm_scratch_bytes) g_norm_scratch = nullptr;
+decltype(&b200q_block_norm_backward) g_norm_backward = nullptr;
+
+bool value_error(const char* what) {
+  PyErr_SetString(PyExc_ValueError, what);
+  return false;
+}
+bool type_error(const char* what) {
+  PyErr_SetString(PyExc_TypeError, what);
+  return false;
+}
+// rows of an operator: 2-D with unit inner stride, rows that do not share memory, sizes that fit the C ABI's integers
+bool check_rows(const at::Tensor& t, const char* name, const c10::Device& dev) {
+  if (t.device() != dev) { PyErr_Format(PyExc_ValueError, "%s must be on the device of the other operands", name); return false; }
+  if (t.dim() != 2 || (t.stride(1) != 1 && t.size(1) > 1)) {
+    PyErr_Format(PyExc_ValueError, "%s must be a 2-D tensor with unit inner stride", name);
+    return false;
+  }
+  if (t.size(0) > INT32_MAX || t.size(1) > INT32_MAX || t.stride(0) > INT32_MAX) {
+    PyErr_Format(PyExc_ValueError, "%s is too large", name);
+    return false;
+  }
+  return true;
+}
+// the row stride; of a single row its length, whatever the tensor says
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+// a contiguous vector of `n` values
+bool check_vector(const at::Tensor& t, const char* name, int64_t n, at::ScalarType type, const c10::Device& dev) {
+  if (t.device() != dev) { PyErr_Format(PyExc_ValueError, "%s must be on the device of the other operands", name); return false; }
+  if (t.scalar_type() != type) { PyErr_Format(PyExc_TypeError, "%s must be %s", name, c10::toString(type)); return false; }
+  if (t.dim() != 1 || t.size(0) != n || !t.is_contiguous()) {
+    PyErr_Format(PyExc_ValueError, "%s must be a contiguous tensor of %lld values", name, (long long)n);
+    return false;
+  }
+  return true;
+}
+bool need_cuda(const at::Tensor& t, const char* op) {
+  if (t.is_cuda()) return true;
+  PyErr_Format(PyExc_ValueError, "%s needs CUDA tensors (there is no CPU path)", op);
+  return false;
+}
+// an optional tensor argument: *t is null where it is None
+bool optional_tensor(PyObject* o, const char* name, const at::Tensor** t) {
+  *t = nullptr;
+  if (o == Py_None) return true;
+  *t = as_tensor(o, name);
+  return *t != nullptr;
+}
+
+// cast_int8(x) -> (out int8 [tokens, hidden], out_sf float32 [tokens])
+PyObject* cast_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 1) { type_error("cast_int8 takes 1 argument"); return nullptr; }
+  const at::Tensor* x = as_tensor(args[0], "x");
+  if (!x || !need_cuda(*x, "per_token_cast_int8") || !check_rows(*x, "x", x->device())) return nullptr;
+  const int act = act_code(x->scalar_type());
+  if (act < 0) { type_error("x must be float16 or bfloat16"); return nullptr; }
+  const c10::Device dev = x->device();
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const int T = (int)x->size(0), H = (int)x->size(1);
+  at::Tensor out = at::detail::empty_cuda({T, H}, at::kChar, dev, std::nullopt);
+  at::Tensor sf = at::detail::empty_cuda({T}, at::kFloat, dev, std::nullopt);
+  if (T > 0) {
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const void* xp = x->const_data_ptr();
+    void *op = out.mutable_data_ptr(), *fp = sf.mutable_data_ptr();
+    const int ldx = (int)row_stride(*x);
+    int st;
+    {
+      const NoGil unlocked;
+      st = g_cast_int(xp, ldx, op, H, static_cast<float*>(fp), T, H, act, stream);
+    }
+    if (st != 0) return raise_status(st);
+  }
+  return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(std::move(out))).get(), THPObjectPtr(THPVariable_Wrap(std::move(sf))).get());
+  END_HANDLE_TH_ERRORS
+}
+
+// igemm(a, b, a_sf, b_sf, bias or None, activation type's code, gated, clamp value or None, out or None) -> out
+PyObject* igemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) { type_error("igemm takes 9 arguments"); return nullptr; }
+  const at::Tensor *a = as_tensor(args[0], "a"), *b = a ? as_tensor(args[1], "b") : nullptr;
+  const at::Tensor *a_sf = b ? as_tensor(args[2], "a_sf") : nullptr, *b_sf = a_sf ? as_tensor(args[3], "b_sf") : nullptr;
+  const at::Tensor *bias, *given;
+  if (!b_sf || !optional_tensor(args[4], "bias", &bias) || !optional_tensor(args[8], "out", &given)) return nullptr;
+  const long act = PyLong_AsLong(args[5]);
+  const int gated = PyObject_IsTrue(args[6]);
+  const bool clamp = args[7] != Py_None;
+  const double clamp_value = clamp ? PyFloat_AsDouble(args[7]) : 0.0;
+  if (PyErr_Occurred()) return nullptr;
+  if (!need_cuda(*a, gated ? "int8_gate_up" : "int8_matmul")) return nullptr;
+  const c10::Device dev = a->device();
+  if (!check_rows(*a, "a", dev) || !check_rows(*b, "b", dev)) return nullptr;
+  if (a->scalar_type() != at::kChar || b->scalar_type() != at::kChar) { type_error("a and b must be int8"); return nullptr; }
+  const int64_t M = a->size(0), K = a->size(1), rows = b->size(0), N = gated ? rows / 2 : rows;
+  if (b->size(1) != K) { value_error("a and b must have rows of the same length"); return nullptr; }
+  if (gated && rows % 2 != 0) { value_error("b must hold as many rows behind the gate's as the gate has"); return nullptr; }
+  if (!check_vector(*a_sf, "a_sf", M, at::kFloat, dev) || !check_vector(*b_sf, "b_sf", rows, at::kFloat, dev)) return nullptr;
+  const at::ScalarType type = act == 1 ? at::kBFloat16 : at::kHalf;
+  if (bias && !check_vector(*bias, "bias", N, type, dev)) return nullptr;
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  if (given) {
+    if (!check_rows(*given, "out", dev)) return nullptr;
+    if (given->scalar_type() != type) { type_error("out must be of out_dtype"); return nullptr; }
+    if (given->size(0) != M || given->size(1) != N) { value_error("out has the wrong shape"); return nullptr; }
+  }
+  at::Tensor out;
+  if (given) out = *given;
+  else out = at::detail::empty_cuda({M, N}, type, dev, std::nullopt);
+  if (M > 0) {
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const at::Tensor ws = workspace_of(dev.index(), stream, 256);
+    const void *ap = a->const_data_ptr(), *bp = b->const_data_ptr(), *biasp = bias ? bias->const_data_ptr() : nullptr;
+    const float *fa = a_sf->const_data_ptr<float>(), *fb = b_sf->const_data_ptr<float>();
+    void *c = out.mutable_data_ptr(), *w = ws.mutable_data_ptr();
+    const int lda = (int)row_stride(*a), ldb = (int)row_stride(*b), ldc = (int)row_stride(out);
+    const size_t ws_bytes = (size_t)ws.numel();
+    int st;
+    {
+      const NoGil unlocked;
+      st = gated ? g_igemm_swiglu(ap, lda, bp, ldb, fa, fb, c, ldc, (int)M, (int)N, (int)K, (int)act, clamp ? 1 : 0, (float)clamp_value,
+                                  w, ws_bytes, stream)
+                 : g_igemm(ap, lda, bp, ldb, fa, fb, biasp, c, ldc, (int)M, (int)N, (int)K, (int)act, w, ws_bytes, stream);
+    }
+    if (st != 0) return raise_status(st);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// The operands that a block norm and its gradient share: (block, residual or None, weight, post weight or None, gate or None,
+// residual scale, eps)
+struct NormOperands {
+  const at::Tensor *block, *residual, *weight, *post, *gate;
+  at::ScalarType residual_type;
+  b200q_block_norm_t c;
+};
+bool parse_norm(PyObject* const* args, const char* op, NormOperands* n) {
+  if (!(n->block = as_tensor(args[0], "block")) || !optional_tensor(args[1], "residual", &n->residual) ||
+      !(n->weight = as_tensor(args[2], "weight")) || !optional_tensor(args[3], "post_weight", &n->post) ||
+      !optional_tensor(args[4], "gate", &n->gate) || !need_cuda(*n->block, op))
+    return false;
+  const double scale = PyFloat_AsDouble(args[5]), eps = PyFloat_AsDouble(args[6]);
+  if (PyErr_Occurred()) return false;
+  const at::ScalarType type = n->block->scalar_type();
+  const c10::Device dev = n->block->device();
+  n->c = b200q_block_norm_t();
+  n->c.act_dtype = act_code(type);
+  if (n->c.act_dtype < 0) return type_error("block must be float16 or bfloat16");
+  if (!check_rows(*n->block, "block", dev)) return false;
+  const int64_t T = n->block->size(0), D = n->block->size(1);
+  n->residual_type = type;
+  if (n->residual) {
+    if (!check_rows(*n->residual, "residual", dev)) return false;
+    n->residual_type = n->residual->scalar_type();
+    if (n->residual_type != type && n->residual_type != at::kFloat)
+      return type_error("residual must be float32 or of the block's type");
+    if (n->residual->size(0) != T || n->residual->size(1) != D) return value_error("residual must have the block's shape");
+    n->c.residual = n->residual->const_data_ptr();
+    n->c.ldr = row_stride(*n->residual);
+  }
+  if (!check_vector(*n->weight, "weight", D, type, dev)) return false;
+  if (n->post && !check_vector(*n->post, "post_weight", D, type, dev)) return false;
+  if (n->gate) {
+    if (n->gate->device() != dev || n->gate->scalar_type() != type)
+      return type_error("gate must be of the block's type and on its device");
+    const int64_t G = n->gate->dim() == 1 ? 1 : n->gate->size(0);
+    if (n->gate->dim() < 1 || n->gate->dim() > 2 || n->gate->size(-1) != D || (D > 1 && n->gate->stride(-1) != 1))
+      return value_error("gate must be [hidden] or [gates, hidden] with unit inner stride");
+    if (G < 1 || T % G != 0) return value_error("gate must have a row for each run of as many tokens");
+    n->c.gate = n->gate->const_data_ptr();
+    n->c.gates = (int32_t)G;
+    n->c.ldg = G > 1 ? n->gate->stride(0) : D;
+  }
+  n->c.block = n->block->const_data_ptr();
+  n->c.weight = n->weight->const_data_ptr();
+  n->c.post_weight = n->post ? n->post->const_data_ptr() : nullptr;
+  n->c.ldb = row_stride(*n->block);
+  n->c.tokens = (int32_t)T;
+  n->c.hidden = (int32_t)D;
+  n->c.residual_f32 = n->residual_type == at::kFloat;
+  n->c.residual_scale = (float)scale;
+  n->c.eps = (float)eps;
+  return true;
+}
+
+// block_norm(the operands, cast) -> (x, new residual), or with the cast (x int8, x_sf float32 [tokens], new residual)
+PyObject* block_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) { type_error("block_norm takes 8 arguments"); return nullptr; }
+  const int cast = PyObject_IsTrue(args[7]);
+  NormOperands n;
+  if (!parse_norm(args, cast ? "block_norm_cast_int8" : "block_norm", &n)) return nullptr;
+  const c10::Device dev = n.block->device();
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const int64_t T = n.c.tokens, D = n.c.hidden;
+  at::Tensor x = at::detail::empty_cuda({T, D}, cast ? at::kChar : n.block->scalar_type(), dev, std::nullopt);
+  at::Tensor fresh = at::detail::empty_cuda({T, D}, n.residual_type, dev, std::nullopt), sf;
+  if (cast) sf = at::detail::empty_cuda({T}, at::kFloat, dev, std::nullopt);
+  if (T > 0) {
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    void *xp = x.mutable_data_ptr(), *rp = fresh.mutable_data_ptr(), *fp = cast ? sf.mutable_data_ptr() : nullptr;
+    int st;
+    {
+      const NoGil unlocked;
+      st = g_norm(&n.c, cast ? nullptr : xp, D, cast ? xp : nullptr, static_cast<float*>(fp), rp, D, stream);
+    }
+    if (st != 0) return raise_status(st);
+  }
+  if (cast)
+    return PyTuple_Pack(3, THPObjectPtr(THPVariable_Wrap(std::move(x))).get(), THPObjectPtr(THPVariable_Wrap(std::move(sf))).get(),
+                        THPObjectPtr(THPVariable_Wrap(std::move(fresh))).get());
+  return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(std::move(x))).get(), THPObjectPtr(THPVariable_Wrap(std::move(fresh))).get());
+  END_HANDLE_TH_ERRORS
+}
+
+// block_norm_backward(the operands, grad_x, grad of the new residual or None)
+//   -> (grad_block, grad_residual or None, grad_weight, grad_post or None, grad_gate or None), the last three float32
+PyObject* block_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) { type_error("block_norm_backward takes 9 arguments"); return nullptr; }
+  NormOperands n;
+  const at::Tensor *dx, *dn;
+  if (!parse_norm(args, "block_norm_backward", &n) || !(dx = as_tensor(args[7], "grad_x")) ||
+      !optional_tensor(args[8], "grad_new_residual", &dn))
+    return nullptr;
+  const c10::Device dev = n.block->device();
+  const int64_t T = n.c.tokens, D = n.c.hidden;
+  if (!check_rows(*dx, "grad_x", dev) || (dn && !check_rows(*dn, "grad_new_residual", dev))) return nullptr;
+  if (dx->scalar_type() != n.block->scalar_type()) { type_error("grad_x must be of the block's type"); return nullptr; }
+  if (dx->size(0) != T || dx->size(1) != D) { value_error("grad_x must have the block's shape"); return nullptr; }
+  if (dn) {
+    // (without a residual the new one has the block's type)
+    if (dn->scalar_type() != n.residual_type) { type_error("grad_new_residual must be of the new residual's type"); return nullptr; }
+    if (dn->size(0) != T || dn->size(1) != D) { value_error("grad_new_residual must have the block's shape"); return nullptr; }
+  }
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  at::Tensor gb = at::detail::empty_cuda({T, D}, n.block->scalar_type(), dev, std::nullopt), gr, gp, gg;
+  at::Tensor gw = at::detail::empty_cuda({D}, at::kFloat, dev, std::nullopt);
+  if (n.residual) gr = at::detail::empty_cuda({T, D}, n.residual_type, dev, std::nullopt);
+  if (n.post) gp = at::detail::empty_cuda({D}, at::kFloat, dev, std::nullopt);
+  if (n.gate) gg = at::detail::empty_cuda(n.gate->sizes(), at::kFloat, dev, std::nullopt);
+  if (T > 0) {
+    const size_t need = g_norm_scratch((int)T, (int)D, n.c.gates);
+    if (need == 0) return raise_status(B200Q_ERR_UNSUPPORTED);
+    const at::Tensor scratch = at::detail::empty_cuda({(int64_t)need}, at::kByte, dev, std::nullopt);
+    void *b = gb.mutable_data_ptr(), *r = n.residual ? gr.mutable_data_ptr() : nullptr, *s = scratch.mutable_data_ptr();
+    float *w = gw.mutable_data_ptr<float>(), *p = n.post ? gp.mutable_data_ptr<float>() : nullptr;
+    float* g = n.gate ? gg.mutable_data_ptr<float>() : nullptr;
+    const void *dxp = dx->const_data_ptr(), *dnp = dn ? dn->const_data_ptr() : nullptr;
+    const int64_t lddx = row_stride(*dx), lddn = dn ? row_stride(*dn) : 0;
+    int st;
+    {
+      const NoGil unlocked;
+      st = g_norm_backward(&n.c, dxp, lddx, dnp, lddn, b, D, r, D, w, p, g, s, need, stream);
+    }
+    if (st != 0) return raise_status(st);
+  } else {
+    for (at::Tensor* t : {&gw, &gp, &gg})
+      if (t->defined() && t->numel()) C10_CUDA_CHECK(cudaMemsetAsync(t->mutable_data_ptr(), 0, (size_t)t->numel() * 4, stream));
+  }
+  auto wrap = [](at::Tensor& t) -> PyObject* {
+    if (t.defined()) return THPVariable_Wrap(std::move(t));
+    Py_RETURN_NONE;
+  };
+  return PyTuple_Pack(5, THPObjectPtr(wrap(gb)).get(), THPObjectPtr(wrap(gr)).get(), THPObjectPtr(wrap(gw)).get(),
+                      THPObjectPtr(wrap(gp)).get(), THPObjectPtr(wrap(gg)).get());
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_int8(per_token_cast_int, igemm, igemm_swiglu, block_norm, block_norm_scratch_bytes, block_norm_backward): addresses
+PyObject* bind_int8(PyObject*, PyObject* args) {
+  unsigned long long f[6];
+  if (!PyArg_ParseTuple(args, "KKKKKK", &f[0], &f[1], &f[2], &f[3], &f[4], &f[5])) return nullptr;
+  g_cast_int = reinterpret_cast<decltype(g_cast_int)>(f[0]);
+  g_igemm = reinterpret_cast<decltype(g_igemm)>(f[1]);
+  g_igemm_swiglu = reinterpret_cast<decltype(g_igemm_swiglu)>(f[2]);
+  g_norm = reinterpret_cast<decltype(g_norm)>(f[3]);
+  g_norm_scratch = reinterpret_cast<decltype(g_norm_scratch)>(f[4]);
+  g_norm_backward = reinterpret_cast<decltype(g_norm_backward)>(f[5]);
+  Py_RETURN_NONE;
+}
+
 // bind(gemm, gemm_host, gemm_swiglu_cast, workspace_bytes, raise_status, raise_unsupported): addresses in
 // libb200q and the Python callables that raise for a status
 PyObject* bind(PyObject*, PyObject* args) {
@@ -392,6 +682,11 @@ PyMethodDef methods[] = {
     {"gate_up_cast", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gate_up_cast)), METH_FASTCALL, nullptr},
     {"workspace", workspace, METH_VARARGS, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
+    {"cast_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(cast_int8)), METH_FASTCALL, nullptr},
+    {"igemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(igemm)), METH_FASTCALL, nullptr},
+    {"block_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(block_norm)), METH_FASTCALL, nullptr},
+    {"block_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(block_norm_backward)), METH_FASTCALL, nullptr},
+    {"bind_int8", bind_int8, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -176,3 +176,72 @@ def swiglu_forward_and_per_token_cast(x: torch.Tensor, num_per_channels: int = 1
             0 if swiglu_clamp_value is None else 1, 0.0 if swiglu_clamp_value is None else float(swiglu_clamp_value),
             _stream_ptr(x.device)))
     return out, sf
+
+
+# ---- 8-bit integers on both sides ----------------------------------------------------------------------
+def per_token_cast_int8(x: torch.Tensor):
+    """x [tokens, hidden] (float16 / bfloat16, CUDA; hidden a multiple of 8) -> (out int8 [tokens, hidden], out_sf float32
+    [tokens]): codes of largest magnitude 127, and the scale that a code stands for.  Activations are cast a row a token,
+    weights [out_features, in_features] a row a channel.  A row of zeros has scale 1; a row with a NaN or an infinity
+    has it as its scale, so that products with it are NaN."""
+    return _lib.native().cast_int8(x)
+
+
+def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_sf: torch.Tensor, b_sf: torch.Tensor, bias: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.float16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """C[M, N] = (A x B^T) * a_sf[:, None] * b_sf + bias for int8 ``a`` [M, K] and ``b`` [N, K] with float32 scales per
+    row of A (token) and per row of B (channel).  The sums are exact (int32); C and ``bias`` are float16 or bfloat16.
+    N and K are multiples of 16, K at most 131056; rows may be strided (by multiples of 16 bytes)."""
+    return _lib.native().igemm(a, b, a_sf, b_sf, bias, act_code(out_dtype), False, None, out)
+
+
+def int8_gate_up(a: torch.Tensor, b: torch.Tensor, a_sf: torch.Tensor, b_sf: torch.Tensor,
+                 out_dtype: torch.dtype = torch.float16, swiglu_clamp_value=None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """A gate_up projection in 8-bit integers with its SwiGLU, in one kernel: ``b`` [2 * hidden, K] holds the gate's rows
+    first; returns silu(gate) * up [M, hidden], clamped as swiglu_forward_and_per_token_cast does where
+    ``swiglu_clamp_value`` is given.  Neither projection is written to memory or rounded on its way."""
+    return _lib.native().igemm(a, b, a_sf, b_sf, None, act_code(out_dtype), True, swiglu_clamp_value, out)
+
+
+def int8_plan(M: int, N: int, K: int, gated: bool = False) -> dict:
+    """The kernel that int8_matmul (int8_gate_up: ``gated``, N its hidden size) takes for a shape."""
+    pl = _lib.IgemmPlan()
+    _lib.check(_lib.load().b200q_igemm_plan(M, N, K, int(gated), ctypes.byref(pl)))
+    return pl.as_dict()
+
+
+# ---- the norms before and after a block ----------------------------------------------------------------
+def block_norm(block: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, *,
+               post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0,
+               eps: float = 1e-6):
+    """What stands between two blocks of a decoder, in one kernel.  For ``block`` [tokens, hidden], the output of one:
+
+        n = rms_norm(block) * post_weight                      (block itself without ``post_weight``)
+        new_residual = residual_scale * residual + gate * n    (None: no residual, no gate)
+        x = rms_norm(new_residual) * weight
+
+    Returns (x, new_residual): the next block's input in the type of ``block`` (float16 / bfloat16) and the residual
+    stream in its own type, which is that or float32.  ``gate`` is [hidden], or [gates, hidden] with a row for each run of
+    tokens / gates rows (one for each sequence of a batch).  hidden is a multiple of 8, at most 16384.  All sums are
+    float32, and x comes from the residual before it is rounded."""
+    return _lib.native().block_norm(block, residual, weight, post_weight, gate, residual_scale, eps, False)
+
+
+def block_norm_cast_int8(block: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, *,
+                         post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                         residual_scale: float = 1.0, eps: float = 1e-6):
+    """block_norm with per_token_cast_int8 of its x in the same kernel: (x int8 [tokens, hidden], x_sf float32 [tokens],
+    new_residual), the operands of int8_matmul and int8_gate_up.  The codes are those of the two calls."""
+    return _lib.native().block_norm(block, residual, weight, post_weight, gate, residual_scale, eps, True)
+
+
+def block_norm_backward(grad_x: torch.Tensor, grad_new_residual: torch.Tensor | None, block: torch.Tensor,
+                        residual: torch.Tensor | None, weight: torch.Tensor, *, post_weight: torch.Tensor | None = None,
+                        gate: torch.Tensor | None = None, residual_scale: float = 1.0, eps: float = 1e-6):
+    """Gradients of block_norm from those of its two outputs (``grad_new_residual`` None: zero):
+    (grad_block, grad_residual, grad_weight, grad_post_weight, grad_gate), None where the operand is.  The first two are of
+    their operand's type, the sums over tokens float32.  Takes the forward call's inputs; nothing else is kept from it.
+    The same inputs give the same bits."""
+    return _lib.native().block_norm_backward(block, residual, weight, post_weight, gate, residual_scale, eps, grad_x,
+                                             grad_new_residual)
