@@ -317,26 +317,31 @@ int b200q_gemm_swiglu_cast(const void* a, int lda, const void* bq, const void* s
  *
  * b200q_igemm_plan names the kernel these calls take; b200q_igemm_planned runs an edited plan.  `workspace` holds the
  * status header (256 bytes, zeroed once, as for the other calls of the stream).  The kernels set up under the end of
- * the stream's previous kernel, and read nothing before that has ended. */
+ * the stream's previous kernel.  With early_b they may read B then: B must not be that kernel's output (weights are not;
+ * codes from a cast right in front of the call are).  Everything else, and with early_b 0 B too, is read after it has ended. */
 typedef struct b200q_igemm_plan {
-  int32_t kernel;  /* 1: pairs of CTAs, 256 rows x 256 product columns a tile; 2: B streamed once (M <= 256) */
+  int32_t kernel;  /* 1: pairs of CTAs, tiles of 256 rows; 2: all rows against a share of the columns in each CTA (M <= 256);
+                      3: mma.sync, B straight from memory (M <= 16) */
   int32_t rows;    /* kernel 2: M rounded up to 16 (output only) */
-  int32_t cluster; /* kernel 2: CTAs that share a column tile's K, 1 .. 8 */
-  int32_t stages;  /* kernel 2: ring slots of 128 bytes of K, 2 .. 12 */
-  int32_t ctas;    /* kernel 1: CTAs, even; kernel 2: output only */
+  int32_t width;   /* kernel 1: product columns of a tile, 256 or 128 (gated: half as many outputs); kernel 2: output columns of
+                      a cluster, a multiple of 16 for each of its CTAs, at most 256 (gated: 128) */
+  int32_t cluster; /* kernel 2: CTAs that share the K of their columns, 1 .. 8 */
+  int32_t stages;  /* kernel 2: ring slots of 128 bytes of K, 1 .. 16 */
+  int32_t ctas;    /* kernel 1: CTAs, even; kernel 3: CTAs; kernel 2: output only */
+  int32_t tail_rows; /* kernel 1: up to 16 last rows that kernel 3 takes in a second launch; else 0 */
 } b200q_igemm_plan_t;
 int b200q_per_token_cast_int(const void* x, int ldx, void* out, int ldo, float* out_sf, int tokens, int hidden,
                              int act_dtype, void* stream);
 int b200q_igemm(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, const void* bias,
-                void* c, int ldc, int M, int N, int K, int act_dtype, void* workspace, size_t workspace_bytes,
-                void* stream);
+                void* c, int ldc, int M, int N, int K, int act_dtype, int early_b, void* workspace,
+                size_t workspace_bytes, void* stream);
 int b200q_igemm_swiglu(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, void* c,
-                       int ldc, int M, int N, int K, int act_dtype, int use_clamp, float clamp_value, void* workspace,
-                       size_t workspace_bytes, void* stream);
+                       int ldc, int M, int N, int K, int act_dtype, int use_clamp, float clamp_value, int early_b,
+                       void* workspace, size_t workspace_bytes, void* stream);
 int b200q_igemm_plan(int M, int N, int K, int gated, b200q_igemm_plan_t* plan);
 int b200q_igemm_planned(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf,
                         const void* bias, void* c, int ldc, int M, int N, int K, int act_dtype, int gated, int use_clamp,
-                        float clamp_value, void* workspace, size_t workspace_bytes, void* stream,
+                        float clamp_value, int early_b, void* workspace, size_t workspace_bytes, void* stream,
                         const b200q_igemm_plan_t* plan);
 
 /* ---- the norms before and after a block, with its gate and residual scale --------------------------------

@@ -117,21 +117,29 @@ def _planned(a, b, a_sf, b_sf, out, gated, **edit):
         setattr(pl, k, v)
     ws = ops.get_workspace("cuda", 256)
     return lib.b200q_igemm_planned(a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), a_sf.data_ptr(), b_sf.data_ptr(), None,
-                                   out.data_ptr(), out.stride(0), M, N, K, ops.act_code(out.dtype), int(gated), 0, 0.0,
+                                   out.data_ptr(), out.stride(0), M, N, K, ops.act_code(out.dtype), int(gated), 0, 0.0, 1,
                                    ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream, ctypes.byref(pl))
 
 
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("M,N,K", [(1, 272, 2064), (40, 400, 1040), (200, 272, 1040)])
+@pytest.mark.parametrize("M,N,K", [(1, 272, 2064), (13, 48, 16), (40, 400, 1040), (130, 144, 304), (200, 272, 1040), (256, 80, 2048),
+                                   (261, 144, 2064), (528, 272, 400)])
 def test_every_plan_gives_the_same_bits(M, N, K, gated):
     """The sums being exact, neither the kernel nor the split of K changes a result."""
     a, b, a_sf, b_sf = _operands(M, N * (2 if gated else 1), K, seed=5)
     first = None
-    edits = [dict(kernel=2, cluster=c, stages=s) for c, s in ((1, 2), (1, 3), (2, 4), (3, 2), (5, 4), (7, 3), (8, 4))]
-    edits += [dict(kernel=1, ctas=2), dict(kernel=1, ctas=6)]
+    edits = [dict(kernel=1, width=w, ctas=c, tail_rows=0) for w, c in ((256, 2), (256, 6), (128, 4), (128, 148))]
+    edits += [dict(kernel=1, width=w, ctas=4, tail_rows=t) for w in (256, 128) for t in (1, 5, 16) if t < M]
+    if M <= 256:
+        edits += [dict(kernel=2, tail_rows=0, width=w * c, cluster=c, stages=s)
+                  for w, c, s in ((16, 1, 1), (48, 1, 3), (80, 1, 3), (128, 1, 2), (16, 2, 4), (64, 2, 1), (16, 3, 2), (32, 4, 3),
+                                  (16, 5, 5), (16, 7, 2), (16, 8, 4), (16, 1, 16))
+                  if c <= -(-K // 128) and (M <= 64 or c < 5 and s < 16)]  # (what shared memory holds)
+    if M <= 16:
+        edits += [dict(kernel=3, tail_rows=0, ctas=c) for c in (1, 3, 300)]
     for edit in edits:
         out = torch.full((M, N), float("nan"), dtype=torch.float16, device="cuda")
-        assert _planned(a, b, a_sf, b_sf, out, gated, **edit) == _lib.ST_OK
+        assert _planned(a, b, a_sf, b_sf, out, gated, **edit) == _lib.ST_OK, edit
         first = out if first is None else first
         assert torch.equal(out, first), edit
     assert ops.device_status(ops.get_workspace("cuda", 256)) == [0, 0, 0, 0]
@@ -140,10 +148,19 @@ def test_every_plan_gives_the_same_bits(M, N, K, gated):
 def test_plans_that_cannot_run_are_refused():
     a, b, a_sf, b_sf = _operands(8, 256, 512)
     out = torch.empty(8, 256, dtype=torch.float16, device="cuda")
-    for edit in (dict(kernel=0), dict(kernel=3), dict(kernel=2, cluster=9), dict(kernel=2, cluster=5), dict(kernel=2, stages=1),
-                 dict(kernel=2, stages=13), dict(kernel=2, cluster=0), dict(kernel=1, ctas=3), dict(kernel=1, ctas=0),
-                 dict(kernel=1, ctas=4096)):
-        assert _planned(a, b, a_sf, b_sf, out, False, **edit) == _lib.ST_UNSUPPORTED, edit
+    good = {1: dict(kernel=1, width=256, ctas=2, tail_rows=0), 2: dict(kernel=2, width=64, cluster=2, stages=2, tail_rows=0),
+            3: dict(kernel=3, ctas=16, tail_rows=0)}
+    for edit in good.values():
+        assert _planned(a, b, a_sf, b_sf, out, False, **edit) == _lib.ST_OK
+    for kernel, edit in ((1, dict(kernel=0)), (1, dict(kernel=4)), (1, dict(width=64)), (1, dict(ctas=3)), (1, dict(ctas=0)),
+                         (1, dict(ctas=4096)), (1, dict(tail_rows=8)), (1, dict(tail_rows=-1)), (2, dict(cluster=9)),
+                         (2, dict(cluster=5)), (2, dict(cluster=0)), (2, dict(stages=0)), (2, dict(stages=17)), (2, dict(width=72)),
+                         (2, dict(width=48)), (2, dict(width=512)), (2, dict(tail_rows=1)), (3, dict(ctas=0)), (3, dict(tail_rows=1))):
+        assert _planned(a, b, a_sf, b_sf, out, False, **{**good[kernel], **edit}) == _lib.ST_UNSUPPORTED, edit
+    a, b, a_sf, b_sf = _operands(17, 256, 512)
+    out = torch.empty(17, 256, dtype=torch.float16, device="cuda")
+    assert _planned(a, b, a_sf, b_sf, out, False, **good[3]) == _lib.ST_UNSUPPORTED
+    assert _planned(a, b, a_sf, b_sf, out, False, **{**good[1], "tail_rows": 17}) == _lib.ST_UNSUPPORTED
 
 
 @pytest.mark.parametrize("M", [3, 300])
@@ -299,10 +316,10 @@ def test_other_streams_and_captured_graphs():
         assert torch.equal(out, want) and torch.equal(out_gated, want_gated)
 
 
-@pytest.mark.parametrize("M,name", [(16, "int8_stream_kernel"), (256, "int8_stream_kernel"), (257, "int8_pair_kernel")])
+@pytest.mark.parametrize("M,name", [(1, "int8_row_kernel"), (17, "int8_stream_kernel"), (128, "int8_stream_kernel"), (300, "int8_pair_kernel")])
 def test_which_kernels_a_layer_launches(M, name):
-    layer = Int8Linear(torch.float16, 512, 1024).cuda()
-    x = torch.zeros(M, 512, dtype=torch.float16, device="cuda")
+    layer = Int8Linear(torch.float16, 1024, 4096).cuda()
+    x = torch.zeros(M, 1024, dtype=torch.float16, device="cuda")
     layer(x), layer.forward_swiglu(x)
     names = launches(lambda: layer(x), lambda: layer.forward_swiglu(x))
     assert ["cast_int_kernel" in n or name in n for n, _ in names] == [True] * 4 and name in names[1][0] and name in names[3][0]

@@ -16,17 +16,24 @@ def lib():
 
 
 def test_plans():
+    """Each plan is one that its kernel can run (what the C ABI demands of an edited one)."""
     for gated in (False, True):
-        cols = 64 if gated else 128
-        for m in (1, 16, 17, 64, 65, 200, 256):
-            for n in (16, 4096, 11008, 28672):
-                for k in (16, 4096, 14336):
+        for m in (1, 8, 9, 16, 17, 64, 65, 200, 256, 257, 272, 273, 4096, 4097, 4113, 100000):
+            for n in (16, 1040, 4096, 11008, 28672, 151936):
+                for k in (16, 144, 4096, 14336, 131056):
                     p = ops.int8_plan(m, n, k, gated)
-                    assert p["kernel"] == 2 and p["rows"] == -(-m // 16) * 16 and 2 <= p["stages"] <= 12
-                    assert 1 <= p["cluster"] <= min(8, -(-k // 128)) and p["ctas"] == -(-n // cols) * p["cluster"]
-        for m in (257, 4097, 100000):
-            p = ops.int8_plan(m, 4096, 4096, gated)
-            assert p["kernel"] == 1 and p["ctas"] % 2 == 0 and 2 <= p["ctas"] <= 148
+                    if p["kernel"] == 1:
+                        assert p["width"] in (128, 256) and p["ctas"] % 2 == 0 and 2 <= p["ctas"] <= 148
+                        assert p["tail_rows"] in (0, m % 256) and 0 <= p["tail_rows"] <= 16 and p["tail_rows"] < m
+                        continue
+                    assert p["tail_rows"] == 0
+                    if p["kernel"] == 3:
+                        assert m <= 16 and 1 <= p["ctas"] <= n // (8 if gated else 16)
+                        continue
+                    assert p["kernel"] == 2 and m <= 256 and p["rows"] == -(-m // 16) * 16 and 2 <= p["stages"] <= 16
+                    assert p["cluster"] in (1, 2, 4, 8) and p["cluster"] <= -(-k // 128)
+                    assert p["width"] % (16 * p["cluster"]) == 0 and 16 <= p["width"] <= (128 if gated else 256)
+                    assert p["ctas"] == -(-n // p["width"]) * p["cluster"]
     for m, n, k in ((1, 24, 128), (1, 128, 24), (1, 16, 131072)):
         with pytest.raises(_lib.B200QError) as e:
             ops.int8_plan(m, n, k)
@@ -38,7 +45,7 @@ def test_plans():
 
 def test_bad_pointers_are_refused_before_a_launch(lib):
     ok = 4096  # (an address that is never used)
-    good = dict(a=ok, lda=128, b=ok, ldb=128, a_sf=ok, b_sf=ok, bias=None, c=ok, ldc=64, M=4, N=64, K=128, act=0, ws=ok, nbytes=256,
+    good = dict(a=ok, lda=128, b=ok, ldb=128, a_sf=ok, b_sf=ok, bias=None, c=ok, ldc=64, M=4, N=64, K=128, act=0, early=1, ws=ok, nbytes=256,
                 stream=None)
     for bad, status in ((dict(a=None), 1), (dict(b=None), 1), (dict(a_sf=None), 1), (dict(b_sf=None), 1), (dict(c=None), 1),
                         (dict(a=ok + 8), 1), (dict(b=ok + 8), 1), (dict(c=ok + 8), 1), (dict(b_sf=ok + 8), 1), (dict(bias=ok + 8), 1),

@@ -65,7 +65,7 @@ class Plan(ctypes.Structure):
 
 class IgemmPlan(ctypes.Structure):
     """b200q_igemm_plan_t of include/b200q.h."""
-    _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "rows", "cluster", "stages", "ctas")]
+    _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "rows", "width", "cluster", "stages", "ctas", "tail_rows")]
 
     def as_dict(self):
         return {n: int(getattr(self, n)) for n, _ in self._fields_}
@@ -112,10 +112,10 @@ SYMBOLS = {
     "b200q_gemm_swiglu_cast": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i,
                                     ctypes.c_float, _vp, _sz, _vp]),
     "b200q_per_token_cast_int": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _vp]),
-    "b200q_igemm": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
-    "b200q_igemm_swiglu": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp]),
+    "b200q_igemm": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "b200q_igemm_swiglu": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp]),
     "b200q_igemm_plan": (_i, [_i, _i, _i, _i, ctypes.POINTER(IgemmPlan)]),
-    "b200q_igemm_planned": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp,
+    "b200q_igemm_planned": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp,
                                  ctypes.POINTER(IgemmPlan)]),
     "b200q_block_norm": (_i, [ctypes.POINTER(BlockNorm), _vp, _ll, _vp, _vp, _vp, _ll, _vp]),
     "b200q_block_norm_scratch_bytes": (_sz, [_i, _i, _i]),

@@ -7,18 +7,23 @@
 namespace b200q {
 
 struct Int8Params {
+  const signed char *a, *b;    // [M, K], [rows, K], row strides lda and ldb (the row kernel; the others have tensor maps of them)
+  long long lda, ldb;
   const float* a_sf;           // [M] scales of the rows of A
   const float* b_sf;           // [columns of the product] scales of the rows of B
   const unsigned short* bias;  // [N] of the output type, or null
   unsigned short* c;           // [M, N], leading dimension ldc
   int* status;                 // workspace status header
   int M, N, K, ldc;            // N: columns of the output (gated: half the rows of B)
-  int kblocks;                 // ceil(K / 128)
+  int kblocks;                 // ceil(K / 128): stages of the pipelines
   int act;                     // type of C and the bias: 0 fp16, 1 bf16
   int use_clamp;               // gated: clamp the gate from above and the other factor on both sides
   float clamp;
   int tiles, m_tiles, n_tiles, m_group;  // pair kernel: output tiles and their raster groups
-  int rows, cluster, stages;   // stream kernel: rows of A rounded up to 16, CTAs that share K, ring slots
+  int rows, width;             // stream kernel: rows of A rounded up to 16, output columns of a CTA (or of a cluster)
+  int cluster, stages;         // CTAs that share K, ring slots
+  int early;                   // stream and row kernels: the kernel before this one does not write B
+  int beside;                  // row kernel: the kernel before this one computes the rows before its own, from the same operands
 };
 
 // api.cu
@@ -34,10 +39,11 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 EncodeTiledFn encode_tiled_fn();
 
 // int8_kernel.cu
-int int8_pair_smem_bytes();
-int int8_stream_smem_bytes(int rows, int stages);
-cudaError_t int8_pair_launch(const Int8Params& p, bool gated, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
-                             int grid, cudaStream_t stream);
+int int8_pair_smem_bytes(int cols);
+int int8_stream_smem_bytes(int M, int b_rows, int cluster, int stages);
+cudaError_t int8_pair_launch(const Int8Params& p, bool gated, int cols, const CUtensorMap& ta, const CUtensorMap& tb,
+                             const CUtensorMap& tc, int grid, cudaStream_t stream);
+cudaError_t int8_row_launch(const Int8Params& p, bool gated, int grid, cudaStream_t stream);
 cudaError_t int8_stream_launch(const Int8Params& p, bool gated, const CUtensorMap& ta, const CUtensorMap& tb, cudaStream_t stream);
 
 }  // namespace b200q

@@ -22,30 +22,90 @@ static int check_igemm(int M, int N, int K) {
 }
 static int igemm_kblocks(int K) { return (K + 127) / 128; }
 
+static int pair_tiles(int M, int N, bool gated, int cols) {
+  const int per = gated ? cols / 2 : cols;
+  return (int)(((long long)M + 255) / 256 * ((N + per - 1) / per));
+}
+// Output columns of a stream kernel's tile with `s` CTAs to a cluster: an equal share of N for all SMs in as few rounds as the
+// tensor core's 256 columns allow, in units of 16 for each CTA.
+static int stream_width(int N, bool gated, int s, int sms) {
+  const int most = (gated ? 128 : 256) / (16 * s) * (16 * s), groups = sms / s;
+  const int rounds = (N + most * groups - 1) / (most * groups);
+  const int share = (N + rounds * groups - 1) / (rounds * groups);
+  return (share + 16 * s - 1) / (16 * s) * (16 * s);
+}
+static int stream_stages(int M, int b_rows, int s, int budget) {
+  int stages = 16;
+  while (stages > 1 && int8_stream_smem_bytes(M, b_rows, s, stages) > budget) --stages;
+  return stages;
+}
+
+// What a call takes, in us, by kernel: fitted to calls of 1 .. 8192 rows x 1024 .. 28672 columns x 128 .. 14336 on a B200, which they
+// meet within some 15 %.  They decide between kernels, so that only their ratios matter.
+constexpr double kHbm = 6465.5e3;  // bytes a us
+
+// Reading B at five sixths of the memory's rate up to eight rows of A (with twice as many, whose loads are as many as B's, at three
+// fifths), but no less than the latency of each round of a CTA.
+static double row_cost(int M, double b_bytes, int rounds) {
+  const double memory = 1.6 + b_bytes / kHbm * (M <= 8 ? 1.2 : 1.62), latency = 0.4 + rounds * (M <= 8 ? 1.5 : 2.0);
+  return memory > latency ? memory : latency;
+}
+
+// A piece of 128 bytes of K takes what the slowest of three takes: reading B, bringing both operands' rows to the SM (121 GB/s a SM),
+// and the tensor core's reading them (about as fast, but whole accumulators' rows of A).  A cluster's exchange goes by its size
+// and rows: 64 x 4096 x 14336 takes 20.1 us alone, 14.5 in pairs, 15.3 in fours; 128 rows 20.7, 17.1, 19.4.
+static double stream_cost(int M, int b_rows, int ctas, int s, int kblocks, const DeviceInfo& di) {
+  const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, rounds = (ctas + di.sm_count - 1) / di.sm_count;
+  const int busy = ctas < di.sm_count ? ctas : di.sm_count;
+  const double tensor = accs * (128 + b_rows) * 1.05e-3, in = (rows + b_rows) * 1.05e-3, memory = 128.0 * b_rows * busy / kHbm * 1.08;
+  const double piece = tensor > in ? (tensor > memory ? tensor : memory) : (in > memory ? in : memory);
+  return 2.8 + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.25 * s + 0.012 * s * M : 0.0) + 0.004 * M;
+}
+
+// A piece of a tile of 256 x 256 takes 0.30 us (0.28 at rest, 0.35 under the power limit), of 256 x 128 two thirds: its operands come
+// through the same SM.  A tile takes no less than its outputs do, 3.1 and 1.9 us (gated 2.6: half
+// of the writers have none of a narrow tile).  Up front, and for the last tile's outputs: 5.6 and 3.9.
+static double pair_cost(int tiles, bool gated, int cols, int kblocks, const DeviceInfo& di) {
+  const int pairs = di.sm_count / 2, rounds = (tiles + pairs - 1) / pairs;
+  const double products = kblocks * (cols == 256 ? 0.30 : 0.195), outputs = cols == 256 ? 3.1 : gated ? 2.6 : 1.9;
+  return (cols == 256 ? 5.6 : 3.9) + products + (rounds - 1) * (products > outputs ? products : outputs);
+}
+
 static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) {
   const DeviceInfo di = device_info();
+  const int kblocks = igemm_kblocks(K);
   *pl = b200q_igemm_plan_t();
-  if (M > kStreamRows) {
-    pl->kernel = 1;
-    pl->rows = 256;
-    pl->cluster = 2;
-    const int tiles = ((M + 255) / 256) * ((N + (gated ? 127 : 255)) / (gated ? 128 : 256));
-    pl->ctas = 2 * (tiles < di.sm_count / 2 ? tiles : di.sm_count / 2);
-    pl->stages = 6;
-    return;
+  double best = 1e30;
+  // Up to 16 rows past the last whole tile may go to the row kernel, beside the pair kernel's last round.
+  const int past = M > 256 && M % 256 <= 16 ? M % 256 : 0;
+  for (int cols = 256; cols >= 128; cols -= 128)
+    for (int tail = 0; tail <= past; tail += past > 0 ? past : 1) {
+      const int tiles = pair_tiles(M - tail, N, gated, cols), items = N / (gated ? 8 : 16), sms = di.sm_count;
+      double cost = pair_cost(tiles, gated, cols, kblocks, di);
+      if (tail > 0) cost += 0.7 * row_cost(tail, (double)(gated ? 2 : 1) * N * K, (items + 2 * sms - 1) / (2 * sms));
+      if (cost >= best) continue;
+      best = cost;
+      *pl = {1, 256, cols, 2, cols == 256 ? 6 : 8, 2 * (tiles < sms / 2 ? tiles : sms / 2), tail};
+    }
+  if (M > kStreamRows) return;
+  for (int s = 1; s <= 8 && 4 * (s - 1) <= kblocks; s *= 2) {
+    const int width = stream_width(N, gated, s, di.sm_count), b_rows = gated ? 2 * width : width;
+    const int ctas = (N + width - 1) / width * s;
+    const double cost = stream_cost(M, b_rows, ctas, s, kblocks, di);
+    if (cost >= best) continue;
+    // half an SM's shared memory where that is depth enough for the length of K: a CTA of the stream's next launch has room next to it
+    // then (126 x 9376 x 704, us with 4 stages / 9 of a whole SM's: 4.6 / 5.4; 100 x 11008 x 4224 with 4 / 8: 14.0 / 11.5)
+    int stages = stream_stages(M, b_rows, s, 113 * 1024);
+    if (stages < (kblocks <= 8 * s ? 3 : 8)) stages = stream_stages(M, b_rows, s, di.max_smem);
+    if (stages < 2) continue;
+    best = cost;
+    *pl = {2, (M + 15) / 16 * 16, width, s, stages, ctas, 0};
   }
-  pl->kernel = 2;
-  pl->rows = (M + 15) / 16 * 16;
-  const int cols = gated ? 64 : 128, tiles = (N + cols - 1) / cols;
-  const int per_sm = pl->rows <= 64 ? 2 : 1;
-  int s = per_sm * di.sm_count / tiles;
-  const int most = (igemm_kblocks(K) + 3) / 4;
-  if (s > most) s = most;
-  pl->cluster = s < 1 ? 1 : s > 8 ? 8 : s;
-  pl->ctas = tiles * pl->cluster;
-  const int budget = per_sm == 2 ? 113 * 1024 : di.max_smem;
-  pl->stages = 12;
-  while (pl->stages > 2 && int8_stream_smem_bytes(pl->rows, pl->stages) > budget) --pl->stages;
+  if (M <= 16) {
+    const int items = N / (gated ? 8 : 16);
+    const double cost = row_cost(M, (double)(gated ? 2 : 1) * N * K, (items + 2 * di.sm_count - 1) / (2 * di.sm_count));
+    if (cost < best) *pl = {3, M, gated ? 8 : 16, 1, 1, items < 2 * di.sm_count ? items : 2 * di.sm_count, 0};
+  }
 }
 
 // 2-D map of 8-bit rows, a box of 128 bytes x `rows`
@@ -60,7 +120,7 @@ static int encode_rows(EncodeTiledFn enc, CUtensorMap* map, const void* base, in
 }
 
 static int run_igemm(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, const void* bias, void* c,
-                     int ldc, int M, int N, int K, int act, bool gated, int use_clamp, float clamp, void* workspace, size_t ws_bytes,
+                     int ldc, int M, int N, int K, int act, bool gated, int use_clamp, float clamp, int early_b, void* workspace, size_t ws_bytes,
                      cudaStream_t stream, const b200q_igemm_plan_t& pl) {
   if (!known_act(act)) return ST_UNSUPPORTED;
   int st = check_igemm(M, N, K);
@@ -74,6 +134,9 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
   const EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return cuda_failed((int)cudaErrorNotSupported);
   Int8Params p = {};
+  p.a = static_cast<const signed char*>(a); p.b = static_cast<const signed char*>(b);
+  p.lda = lda; p.ldb = ldb;
+  p.early = early_b ? 1 : 0;
   p.a_sf = a_sf; p.b_sf = b_sf;
   p.bias = static_cast<const unsigned short*>(bias);
   p.c = static_cast<unsigned short*>(c);
@@ -86,29 +149,43 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
   const long long b_rows = gated ? 2ll * N : N;
   CUtensorMap ta, tb, tc;
   cudaError_t e;
-  if (pl.kernel == 1) {
-    st = encode_rows(enc, &ta, a, K, M, lda, 128);
-    if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, 128);
+  if (pl.kernel == 3) {
+    e = int8_row_launch(p, gated, pl.ctas, stream);
+  } else if (pl.kernel == 1) {
+    const int pc = pl.width;
+    p.M = M - pl.tail_rows;
+    st = encode_rows(enc, &ta, a, K, p.M, lda, 128);
+    if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, pc / 2);
     if (st != ST_OK) return st;
-    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)p.M};
     const cuuint64_t strides[1] = {(cuuint64_t)ldc * 2};
-    const cuuint32_t box[2] = {64u, 128u}, steps[2] = {1u, 1u};
+    const cuuint32_t box[2] = {64u, 32u}, steps[2] = {1u, 1u};
     const CUresult r = enc(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, c, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return cuda_failed((int)r);
-    p.m_tiles = (int)(((long long)M + 255) / 256);
-    p.n_tiles = (N + (gated ? 127 : 255)) / (gated ? 128 : 256);
+    p.m_tiles = (int)(((long long)p.M + 255) / 256);
+    const int per = gated ? pc / 2 : pc;
+    p.n_tiles = (N + per - 1) / per;
     if ((long long)p.m_tiles * p.n_tiles > 0x7fffffffll) return ST_UNSUPPORTED;
     p.tiles = p.m_tiles * p.n_tiles;
     // rows of A that stay in the L2 cache while the columns of B stream past them: about 32 MB
     const long long fit = (32ll << 20) / (256ll * K);
     p.m_group = (int)(fit < 1 ? 1 : fit > p.m_tiles ? p.m_tiles : fit);
-    e = int8_pair_launch(p, gated, ta, tb, tc, pl.ctas, stream);
+    e = int8_pair_launch(p, gated, pc, ta, tb, tc, pl.ctas, stream);
+    if (e == cudaSuccess && pl.tail_rows > 0) {
+      p.a += (size_t)p.M * lda;
+      p.a_sf += p.M;
+      p.c += (size_t)p.M * ldc;
+      p.M = pl.tail_rows;
+      p.beside = 1;
+      const int items = N / (gated ? 8 : 16), most = 2 * device_info().sm_count;
+      e = int8_row_launch(p, gated, items < most ? items : most, stream);
+    }
   } else {
     st = encode_rows(enc, &ta, a, K, M, lda, pl.rows);
-    if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, gated ? 64 : 128);
+    if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, pl.width);
     if (st != ST_OK) return st;
-    p.rows = pl.rows; p.cluster = pl.cluster; p.stages = pl.stages;
+    p.rows = pl.rows; p.width = pl.width; p.cluster = pl.cluster; p.stages = pl.stages;
     p.tiles = pl.ctas / pl.cluster;
     e = int8_stream_launch(p, gated, ta, tb, stream);
   }
@@ -119,15 +196,20 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
 static bool igemm_plan_ok(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) {
   const DeviceInfo di = device_info();
   if (pl->kernel == 1) {
+    if (pl->width != 128 && pl->width != 256) return false;
+    if (pl->tail_rows < 0 || pl->tail_rows > 16 || pl->tail_rows >= M) return false;
     if (pl->ctas < 2 || pl->ctas % 2 != 0 || pl->ctas > di.sm_count) return false;
-    return int8_pair_smem_bytes() <= di.max_smem;
+    return int8_pair_smem_bytes(pl->width) <= di.max_smem;
   }
+  if (pl->tail_rows != 0) return false;
+  if (pl->kernel == 3) return M <= 16 && pl->ctas >= 1 && pl->ctas <= 8 * di.sm_count;
   if (pl->kernel != 2 || M > kStreamRows) return false;
   pl->rows = (M + 15) / 16 * 16;
-  const int cols = gated ? 64 : 128;
   if (pl->cluster < 1 || pl->cluster > 8 || pl->cluster > igemm_kblocks(K)) return false;
-  pl->ctas = (N + cols - 1) / cols * pl->cluster;
-  return pl->stages >= 2 && pl->stages <= 12 && int8_stream_smem_bytes(pl->rows, pl->stages) <= di.max_smem;
+  if (pl->width < 16 || pl->width > (gated ? 128 : 256) || pl->width % (16 * pl->cluster) != 0) return false;
+  pl->ctas = (N + pl->width - 1) / pl->width * pl->cluster;
+  return pl->stages >= 1 && pl->stages <= 16 &&
+         int8_stream_smem_bytes(M, gated ? 2 * pl->width : pl->width, pl->cluster, pl->stages) <= di.max_smem;
 }
 
 // ---- row-wise kernels -------------------------------------------------------------------------------------
@@ -161,37 +243,37 @@ int b200q_igemm_plan(int M, int N, int K, int gated, b200q_igemm_plan_t* plan) {
 }
 
 int b200q_igemm(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, const void* bias, void* c, int ldc,
-                int M, int N, int K, int act_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+                int M, int N, int K, int act_dtype, int early_b, void* workspace, size_t workspace_bytes, void* stream) {
   int st = check_igemm(M, N, K);
   if (st != ST_OK) return st;
   b200q_igemm_plan_t pl;
   plan_igemm(M, N, K, false, &pl);
-  return run_igemm(a, lda, b, ldb, a_sf, b_sf, bias, c, ldc, M, N, K, act_dtype, false, 0, 0.f, workspace, workspace_bytes,
+  return run_igemm(a, lda, b, ldb, a_sf, b_sf, bias, c, ldc, M, N, K, act_dtype, false, 0, 0.f, early_b, workspace, workspace_bytes,
                    static_cast<cudaStream_t>(stream), pl);
 }
 
 int b200q_igemm_swiglu(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, void* c, int ldc, int M,
-                       int N, int K, int act_dtype, int use_clamp, float clamp_value, void* workspace, size_t workspace_bytes,
-                       void* stream) {
+                       int N, int K, int act_dtype, int use_clamp, float clamp_value, int early_b, void* workspace,
+                       size_t workspace_bytes, void* stream) {
   int st = check_igemm(M, N, K);
   if (st != ST_OK) return st;
   if (N > 0x7fffffff / 2) return ST_UNSUPPORTED;
   b200q_igemm_plan_t pl;
   plan_igemm(M, N, K, true, &pl);
-  return run_igemm(a, lda, b, ldb, a_sf, b_sf, nullptr, c, ldc, M, N, K, act_dtype, true, use_clamp, clamp_value, workspace,
-                   workspace_bytes, static_cast<cudaStream_t>(stream), pl);
+  return run_igemm(a, lda, b, ldb, a_sf, b_sf, nullptr, c, ldc, M, N, K, act_dtype, true, use_clamp, clamp_value, early_b,
+                   workspace, workspace_bytes, static_cast<cudaStream_t>(stream), pl);
 }
 
 int b200q_igemm_planned(const void* a, int lda, const void* b, int ldb, const float* a_sf, const float* b_sf, const void* bias, void* c,
-                        int ldc, int M, int N, int K, int act_dtype, int gated, int use_clamp, float clamp_value, void* workspace,
-                        size_t workspace_bytes, void* stream, const b200q_igemm_plan_t* plan) {
+                        int ldc, int M, int N, int K, int act_dtype, int gated, int use_clamp, float clamp_value,
+                        int early_b, void* workspace, size_t workspace_bytes, void* stream, const b200q_igemm_plan_t* plan) {
   int st = check_igemm(M, N, K);
   if (st != ST_OK) return st;
   if (!plan || (gated && (bias || N > 0x7fffffff / 2))) return ST_INVALID_ARG;
   b200q_igemm_plan_t pl = *plan;
   if (!igemm_plan_ok(M, N, K, gated != 0, &pl)) return ST_UNSUPPORTED;
-  return run_igemm(a, lda, b, ldb, a_sf, b_sf, bias, c, ldc, M, N, K, act_dtype, gated != 0, use_clamp, clamp_value, workspace,
-                   workspace_bytes, static_cast<cudaStream_t>(stream), pl);
+  return run_igemm(a, lda, b, ldb, a_sf, b_sf, bias, c, ldc, M, N, K, act_dtype, gated != 0, use_clamp, clamp_value, early_b,
+                   workspace, workspace_bytes, static_cast<cudaStream_t>(stream), pl);
 }
 
 int b200q_per_token_cast_int(const void* x, int ldx, void* out, int ldo, float* out_sf, int tokens, int hidden, int act_dtype,

@@ -84,6 +84,7 @@ struct StreamBuffers {
   at::Tensor workspace;
   at::Tensor staging[2][2];
   std::vector<at::Tensor> superseded;
+  const char *cast_begin = nullptr, *cast_end = nullptr;  // codes that the stream's latest cast writes, see codes_written
   std::mutex host_call;  // a host call is several operations on one staging pair: one thread's at a time
 };
 std::mutex g_mutex;
@@ -423,6 +424,25 @@ bool optional_tensor(PyObject* o, const char* name, const at::Tensor** t) {
   return *t != nullptr;
 }
 
+// A product may read its operand B (weights) before the kernel in front of it has ended, unless that one writes it.  What writes
+// int8 codes here are the casts, and each kernel of these operators lets the next one start only when the one before itself has
+// ended: so it is the stream's latest cast that matters.  Its outputs are noted until a product has been launched behind it (which
+// waits for it and for everything before).
+void codes_written(int device, cudaStream_t stream, const void* codes, int64_t bytes) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  StreamBuffers& b = buffers_of(device, stream);
+  b.cast_begin = static_cast<const char*>(codes);
+  b.cast_end = b.cast_begin + bytes;
+}
+bool settled(int device, cudaStream_t stream, const void* operand, int64_t bytes) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  StreamBuffers& b = buffers_of(device, stream);
+  const char* p = static_cast<const char*>(operand);
+  const bool apart = b.cast_begin == nullptr || p >= b.cast_end || p + bytes <= b.cast_begin;
+  b.cast_begin = b.cast_end = nullptr;
+  return apart;
+}
+
 // cast_int8(x) -> (out int8 [tokens, hidden], out_sf float32 [tokens])
 PyObject* cast_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -441,6 +461,7 @@ PyObject* cast_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const void* xp = x->const_data_ptr();
     void *op = out.mutable_data_ptr(), *fp = sf.mutable_data_ptr();
     const int ldx = (int)row_stride(*x);
+    codes_written(dev.index(), stream, op, (int64_t)T * H);
     int st;
     {
       const NoGil unlocked;
@@ -492,12 +513,13 @@ PyObject* igemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     void *c = out.mutable_data_ptr(), *w = ws.mutable_data_ptr();
     const int lda = (int)row_stride(*a), ldb = (int)row_stride(*b), ldc = (int)row_stride(out);
     const size_t ws_bytes = (size_t)ws.numel();
+    const int early = settled(dev.index(), stream, bp, (rows - 1) * ldb + K) ? 1 : 0;
     int st;
     {
       const NoGil unlocked;
       st = gated ? g_igemm_swiglu(ap, lda, bp, ldb, fa, fb, c, ldc, (int)M, (int)N, (int)K, (int)act, clamp ? 1 : 0, (float)clamp_value,
-                                  w, ws_bytes, stream)
-                 : g_igemm(ap, lda, bp, ldb, fa, fb, biasp, c, ldc, (int)M, (int)N, (int)K, (int)act, w, ws_bytes, stream);
+                                  early, w, ws_bytes, stream)
+                 : g_igemm(ap, lda, bp, ldb, fa, fb, biasp, c, ldc, (int)M, (int)N, (int)K, (int)act, early, w, ws_bytes, stream);
     }
     if (st != 0) return raise_status(st);
   }
@@ -577,6 +599,7 @@ PyObject* block_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (T > 0) {
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
     void *xp = x.mutable_data_ptr(), *rp = fresh.mutable_data_ptr(), *fp = cast ? sf.mutable_data_ptr() : nullptr;
+    if (cast) codes_written(dev.index(), stream, xp, T * D);
     int st;
     {
       const NoGil unlocked;

@@ -8,6 +8,13 @@
 
 namespace b200q {
 
+// The kernel before this one in the stream has ended; the one behind it may set up now, and no earlier: what it reads before this
+// one has ended (weights) is then at least one kernel old.
+__device__ __forceinline__ void start_behind() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 template <int ACT>
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -91,33 +98,40 @@ __device__ __forceinline__ void row_reduce(float (&v)[N], float* slots, bool war
 // ---- per-token int8 cast --------------------------------------------------------------------------------
 // m = max |x| of the row (as bits, so that a NaN is the largest);  out_sf = m / 127,  out = rint(x * (127 / m)), quotients and
 // product rounded to fp32.  Rows of m < 2^-100 count as zero (127 / m would leave the range of fp32): codes 0, scale 1.  A row
-// with a NaN or an infinity gets it as its scale, and codes 0 there: products with it are NaN, as they would be.
+// with a NaN or an infinity gets it as its scale, and codes 0: products with it are NaN, as they would be.
 __device__ __forceinline__ void int8_scale(float top, float* sf, float* inv) {
   const bool zero = top < 0x1p-100f;
   *sf = zero ? 1.0f : __fdiv_rn(top, 127.0f);
   *inv = zero ? 0.0f : __fdiv_rn(127.0f, top);
+  if (!(top < __int_as_float(0x7f800000))) *inv = 0.0f;
 }
+// Codes of eight values: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves its low byte in the sum's.
 __device__ __forceinline__ uint2 int8_codes(const float (&f)[8], float inv) {
-  uint32_t w[2] = {0, 0};
+  uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    int q;
-    asm("cvt.rni.s32.f32 %0, %1;" : "=r"(q) : "f"(__fmul_rn(f[i], inv)));  // (NaN becomes 0)
-    w[i >> 2] |= ((uint32_t)q & 0xffu) << (8 * (i & 3));
+  for (int h = 0; h < 2; ++h) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[4 * h + i], inv), 12582912.0f));
+    w[h] = inv != 0.0f ? __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) : 0u;
   }
   return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ float abs_top(float top, const float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(f[i]) & 0x7fffffffu));
-  return top;
+// The largest magnitude among 16-bit values, as bits (either type's order like integers, NaN above infinity), two at a time.
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, const uint4& v) {
+  top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
+  return __vmaxu2(__vmaxu2(top, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+}
+template <int ACT>
+__device__ __forceinline__ float top_value(uint32_t top) {
+  const uint32_t one = max(top & 0xffffu, top >> 16);
+  return ACT == 0 ? __half2float(__ushort_as_half((unsigned short)one)) : __uint_as_float(one << 16);
 }
 
 template <int ACT, int V>
 __global__ void __launch_bounds__(1024) cast_int_kernel(const CastIntParams p, const int warp_rows) {
   __shared__ float slots[32];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  start_behind();
   const bool warp_row = warp_rows != 0;
   const int tpr = warp_row ? 32 : blockDim.x, me = warp_row ? threadIdx.x & 31 : threadIdx.x;
   const int t = warp_row ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -125,23 +139,16 @@ __global__ void __launch_bounds__(1024) cast_int_kernel(const CastIntParams p, c
   const int nvec = p.D / 8;
   const uint4* row = reinterpret_cast<const uint4*>(p.x + (size_t)t * p.ldx);
   uint4 keep[V];
-  float top[1] = {0.f};
+  uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = me + i * tpr;
     keep[i] = v < nvec ? row[v] : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float f[8];
-    unpack8<ACT>(keep[i], f);
-    top[0] = abs_top(top[0], f);
-  }
-  for (int v = me + V * tpr; v < nvec; v += tpr) {  // (what does not stay in registers is read again)
-    float f[8];
-    unpack8<ACT>(row[v], f);
-    top[0] = abs_top(top[0], f);
-  }
+  for (int i = 0; i < V; ++i) bits = top_bits(bits, keep[i]);
+  for (int v = me + V * tpr; v < nvec; v += tpr) bits = top_bits(bits, row[v]);  // (what does not stay in registers is read again)
+  float top[1] = {top_value<ACT>(bits)};
   row_reduce<1, true>(top, slots, warp_row);
   float sf, inv;
   int8_scale(top[0], &sf, &inv);
@@ -165,8 +172,7 @@ __global__ void __launch_bounds__(1024) cast_int_kernel(const CastIntParams p, c
 template <int ACT, bool F32, int V>
 __global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const int warp_rows) {
   __shared__ float slots[3][32];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  start_behind();
   const bool warp_row = warp_rows != 0;
   const int tpr = warp_row ? 32 : blockDim.x, me = warp_row ? threadIdx.x & 31 : threadIdx.x;
   const int t = warp_row ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -226,7 +232,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const in
   }
   row_reduce<1, false>(s, slots[1], warp_row);
   const float inv = rsqrtf(s[0] * inv_d + p.eps);
-  float top[1] = {0.f};
+  uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = me + i * tpr;
@@ -240,11 +246,12 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const in
         *reinterpret_cast<uint4*>(p.x + t * p.ldx + v * 8) = x;
       } else {
         unpack8<ACT>(x, r[i]);  // what is cast is the rounded x: the codes are those of a cast of it
-        top[0] = abs_top(top[0], r[i]);
+        bits = top_bits(bits, x);
       }
     }
   }
   if (!p.x) {
+    float top[1] = {top_value<ACT>(bits)};
     row_reduce<1, true>(top, slots[2], warp_row);
     float sf, qinv;
     int8_scale(top[0], &sf, &qinv);
