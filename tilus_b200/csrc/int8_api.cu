@@ -215,20 +215,6 @@ static bool igemm_plan_ok(int M, int N, int K, bool gated, b200q_igemm_plan_t* p
 // ---- row-wise kernels -------------------------------------------------------------------------------------
 static const int kNormMaxD = 16384;
 
-// CTAs of the gradient's launch: whole rounds of the GPU, split evenly over the gates
-static void norm_backward_grid(int T, int D, int gates, int* grid, int* per_gate) {
-  const int sms = device_info().sm_count, nvec = D / 8;
-  const int most = sms * (nvec <= 128 ? 4 : nvec <= 256 ? 2 : 1);
-  const int tokens = T / gates;
-  if (gates >= most) {
-    *per_gate = 1;
-    *grid = most;
-  } else {
-    *per_gate = most / gates < tokens ? most / gates : tokens;
-    *grid = gates * *per_gate;
-  }
-}
-
 }  // namespace b200q
 
 using namespace b200q;
@@ -335,9 +321,10 @@ int b200q_block_norm(const b200q_block_norm_t* a, void* x, long long ldx, void* 
 
 size_t b200q_block_norm_scratch_bytes(int tokens, int hidden, int gates) {
   if (tokens < 1 || hidden < 8 || hidden % 8 != 0 || hidden > kNormMaxD || gates < 0 || (gates > 0 && tokens % gates != 0)) return 0;
-  int grid, per_gate;
-  norm_backward_grid(tokens, hidden, gates > 0 ? gates : 1, &grid, &per_gate);
-  return (size_t)3 * grid * hidden * sizeof(float);
+  NormBackwardParams p;
+  const DeviceInfo di = device_info();
+  norm_backward_shape(hidden, false, gates > 0 ? gates : 1, tokens / (gates > 0 ? gates : 1), di.sm_count, di.max_smem, &p);
+  return (size_t)3 * p.grid * hidden * sizeof(float);
 }
 
 int b200q_block_norm_backward(const b200q_block_norm_t* a, const void* grad_x, long long lddx, const void* grad_new, long long lddn,
@@ -369,7 +356,8 @@ int b200q_block_norm_backward(const b200q_block_norm_t* a, const void* grad_x, l
   p.T = a->tokens; p.D = a->hidden;
   p.gates = a->gates > 0 ? a->gates : 1;
   p.tokens_per_gate = a->tokens / p.gates;
-  norm_backward_grid(p.T, p.D, p.gates, &p.grid, &p.ctas_per_gate);
+  const DeviceInfo di = device_info();
+  norm_backward_shape(p.D, a->residual_f32 != 0, p.gates, p.tokens_per_gate, di.sm_count, di.max_smem, &p);
   p.ldb = a->ldb; p.ldr = a->ldr; p.ldg = a->ldg;
   p.lddx = lddx; p.lddn = lddn; p.lddb = lddb; p.lddr = lddr;
   p.scale = a->residual_scale; p.eps = a->eps;

@@ -35,10 +35,12 @@ struct NormBackwardParams {
   float* partial;                   // [CTAs][2 or 3][D]
   int T, D, gates, tokens_per_gate;
   int ctas_per_gate, grid;          // CTAs that share a gate's rows; several gates to a CTA where it is 1
+  int threads, vectors, stages, smem;  // threads of a row, its vectors of a thread, rows in shared memory and their bytes
   long long ldb, ldr, ldg, lddx, lddn, lddb, lddr;
   float scale, eps;
 };
 
+void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gate, int sms, int max_smem, NormBackwardParams* p);
 cudaError_t cast_int_launch(const CastIntParams& p, int act, cudaStream_t stream);
 cudaError_t norm_launch(const NormParams& p, int act, bool residual_f32, cudaStream_t stream);
 cudaError_t norm_backward_launch(const NormBackwardParams& p, int act, bool residual_f32, cudaStream_t stream);

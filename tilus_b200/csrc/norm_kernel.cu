@@ -266,172 +266,250 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const in
 
 // ---- its gradient ---------------------------------------------------------------------------------------
 // With s1, s2 the inverse deviations of the two norms, recomputed from the inputs (which have to be read anyway):
-//   bh = block s1, n = bh post;  r = scale residual + gate n;  xh = r s2;  e = grad_x weight
-//   dr = grad_new + s2 (e - xh mean(e xh));   grad_residual = scale dr;   dn = gate dr
-//   grad_block = s1 (f - bh mean(f bh)) with f = dn post   (dn without a norm after the block)
-//   grad_weight = sum grad_x xh,  grad_post = sum dn bh,  grad_gate = sum dr n   over the rows (of the gate)
-// A CTA takes a run of rows of one gate and keeps its share of the three sums in registers; a second kernel adds the CTAs' shares
-// in a fixed order, so that a call gives the same bits each time.
+//   bh = block s1, q = bh post gate (= gate n);  r = scale residual + q;  xh = r s2;  e = grad_x weight
+//   dr = grad_new + s2 (e - xh mean(e xh));   grad_residual = scale dr
+//   grad_block = s1 (dr post gate - bh mean(dr q))      (dr gate without a norm after the block)
+//   grad_weight = sum grad_x xh;   with S = sum dr bh over the rows of a gate: grad_gate = post S, grad_post = sum of gate S
+// dr is linear in e and r, so that mean(dr q) follows from the row's sums of q grad_new, q e and q r, which can be taken together with
+// those of r r and e r, and with the next row's sum of block block: one reduction over the CTA for each row.
+//
+// A CTA takes a run of rows of one gate and keeps its share of the sums over rows in registers; a second kernel adds the CTAs' shares
+// in a fixed order, so that a call gives the same bits each time.  Rows are copied to shared memory ahead of their turn
+// (cp.async, each thread what it will read itself, so that nobody waits for anybody's copies): with a row at a time in registers and three
+// reductions 8192 x 5120 took 386 us, of a floor of 117.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_wait(int pending) {  // all but the latest `pending` groups have landed
+  if (pending <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 2;" ::: "memory");
+}
+
+// The sums of eight values over the CTA's threads, in every thread.  Halving exchanges: after the steps over 16, 8 and 4 lanes a lane
+// holds one value, lane >> 2; so a warp's part takes 9 shuffles instead of 40.  `slots`: 8 words a warp, of two sets in turn.
+__device__ __forceinline__ void sums8(float (&v)[8], float* slots) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float give = lane & 16 ? v[i] : v[i + 4], mine = lane & 16 ? v[i + 4] : v[i];
+    v[i] = mine + __shfl_xor_sync(0xffffffffu, give, 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float give = lane & 8 ? v[i] : v[i + 2], mine = lane & 8 ? v[i + 2] : v[i];
+    v[i] = mine + __shfl_xor_sync(0xffffffffu, give, 8);
+  }
+  const float give = lane & 4 ? v[0] : v[1], mine = lane & 4 ? v[1] : v[0];
+  float x = mine + __shfl_xor_sync(0xffffffffu, give, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 2);
+  x += __shfl_xor_sync(0xffffffffu, x, 1);
+  if ((lane & 3) == 0) slots[warp * 8 + (lane >> 2)] = x;
+  __syncthreads();
+  x = 0.f;
+  for (int w = lane >> 3; w < warps; w += 4) x += slots[w * 8 + (lane & 7)];
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  x += __shfl_xor_sync(0xffffffffu, x, 16);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __shfl_sync(0xffffffffu, x, i);
+}
+
+// V: vectors of eight channels to a thread.  Up to two, the weights of a thread's channels stay in registers too.
 template <int ACT, bool F32, int V>
 __global__ void __launch_bounds__(512) norm_backward_kernel(const NormBackwardParams p) {
-  __shared__ float slots[3][64];
+  extern __shared__ __align__(16) unsigned char rows_smem[];
+  __shared__ float slots[2][128], slots_block[512 / 32];
+  constexpr int WIDE = F32 ? 2 : 1, UNITS = 2 + 2 * WIDE;  // 16-byte units of a vector: block, grad_x, residual, grad_new
+  constexpr bool KEEP = V <= 2;
+  start_behind();
   const int me = threadIdx.x, tpr = blockDim.x, nvec = p.D / 8;
   const float inv_d = 1.0f / (float)p.D;
-  uint4 weight[V], post[V], gate[V];
-  float gw[V][8], gp[V][8], gg[V][8];
-  const uint4 none = make_uint4(0, 0, 0, 0);
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(rows_smem) + (uint32_t)me * 16u;
+  // the unit u of vector i in stage s
+  auto at = [&](int s, int u, int i) { return mine + (uint32_t)(((s * UNITS + u) * V + i) * tpr) * 16u; };
+  auto wide_at = [&](int s, int u, int i, float (&f)[8]) {
+    Wide<ACT, F32> w;
+#pragma unroll
+    for (int h = 0; h < WIDE; ++h) w.v[h] = lds_u4(at(s, u + h, i));
+    w.get(f);
+  };
+  // The weights of a vector's channels: of the second norm, and of what stands in front of the residual (post and gate together)
+  auto load_w = [&](int i, float (&w)[8]) {
+    const int v = me + i * tpr;
+    unpack8<ACT>(v < nvec ? *reinterpret_cast<const uint4*>(p.weight + v * 8) : make_uint4(0, 0, 0, 0), w);
+  };
+  auto load_pg = [&](int g, int i, float (&pg)[8]) {
+    const int v = me + i * tpr;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) pg[k] = 1.f;
+    float x[8];
+    if (p.post && v < nvec) unpack8<ACT>(*reinterpret_cast<const uint4*>(p.post + v * 8), pg);
+    if (p.gate && v < nvec) {
+      unpack8<ACT>(*reinterpret_cast<const uint4*>(p.gate + g * p.ldg + v * 8), x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) pg[k] *= x[k];
+    }
+  };
+  float kept_w[KEEP ? V : 1][8], kept_pg[KEEP ? V : 1][8];
+  float gw[V][8], S[V][8];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int v = me + i * tpr;
-    weight[i] = v < nvec ? *reinterpret_cast<const uint4*>(p.weight + v * 8) : none;
-    post[i] = p.post && v < nvec ? *reinterpret_cast<const uint4*>(p.post + v * 8) : none;
+    if constexpr (KEEP) load_w(i, kept_w[i]);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) gw[i][k] = gp[i][k] = 0.f;
+    for (int k = 0; k < 8; ++k) gw[i][k] = 0.f;
   }
+  // Three stages and more: a row's reduction takes the next row's sum of block block along, whose copies have landed by then.
+  const bool ahead = p.stages >= 3;
   const int part = (int)(blockIdx.x % p.ctas_per_gate), stride = (int)(gridDim.x / p.ctas_per_gate);
-  for (int g = blockIdx.x / p.ctas_per_gate; g < p.gates; g += stride) {
+  bool first_gate = true;
+  for (int g = blockIdx.x / p.ctas_per_gate; g < p.gates; g += stride, first_gate = false) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int v = me + i * tpr;
-      gate[i] = p.gate && v < nvec ? *reinterpret_cast<const uint4*>(p.gate + g * p.ldg + v * 8) : none;
+      if constexpr (KEEP) load_pg(g, i, kept_pg[i]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) gg[i][k] = 0.f;
+      for (int k = 0; k < 8; ++k) S[i][k] = 0.f;
     }
     const long long t0 = (long long)g * p.tokens_per_gate;
     const int r0 = (int)((long long)p.tokens_per_gate * part / p.ctas_per_gate);
-    const int r1 = (int)((long long)p.tokens_per_gate * (part + 1) / p.ctas_per_gate);
-    for (long long t = t0 + r0; t < t0 + r1; ++t) {
-      uint4 block[V], dx[V];
-      Wide<ACT, F32> res[V], dn[V];
+    const int rows = (int)((long long)p.tokens_per_gate * (part + 1) / p.ctas_per_gate) - r0;
+    auto fetch = [&](int n) {  // row n of this run, to stage n % stages
+      if (n < rows) {
+        const long long t = t0 + r0 + n;
+        const int s = n % p.stages;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int v = me + i * tpr;
+          if (v < nvec) {
+            copy16(at(s, 0, i), p.block + t * p.ldb + v * 8);
+            copy16(at(s, 1, i), p.grad_x + t * p.lddx + v * 8);
+#pragma unroll
+            for (int h = 0; h < WIDE; ++h) {
+              if (p.residual) copy16(at(s, 2 + h, i), static_cast<const char*>(p.residual) + (t * p.ldr + v * 8) * (F32 ? 4 : 2) + h * 16);
+              if (p.grad_new) copy16(at(s, 2 + WIDE + h, i), static_cast<const char*>(p.grad_new) + (t * p.lddn + v * 8) * (F32 ? 4 : 2) + h * 16);
+            }
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto block_square = [&](int s) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float b[8];
+        unpack8<ACT>(lds_u4(at(s, 0, i)), b);
+        if (me + i * tpr < nvec)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x += b[k] * b[k];
+      }
+      return x;
+    };
+    for (int n = 0; n < p.stages - 1; ++n) fetch(n);
+    float s1 = 1.f;
+    if (ahead && p.post && rows > 0) {
+      copies_wait(p.stages - 2);
+      float x[1] = {block_square(0)};
+      row_reduce<1, false>(x, slots_block, false);
+      s1 = rsqrtf(x[0] * inv_d + p.eps);
+    }
+    for (int n = 0; n < rows; ++n) {
+      const int s = n % p.stages;
+      fetch(n + p.stages - 1);
+      copies_wait(ahead ? p.stages - 2 : p.stages - 1);
+      if (!ahead && p.post) {
+        float x[1] = {block_square(s)};
+        row_reduce<1, false>(x, slots_block, false);
+        s1 = rsqrtf(x[0] * inv_d + p.eps);
+      }
+      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      float kept_r[1][8];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (me + i * tpr < nvec) {
+          float b[8], d[8], res[8], dn[8], w[8], pg[8];
+          unpack8<ACT>(lds_u4(at(s, 0, i)), b);
+          unpack8<ACT>(lds_u4(at(s, 1, i)), d);
+          if (p.residual) wide_at(s, 2, i, res);
+          if (p.grad_new) wide_at(s, 2 + WIDE, i, dn);
+          if constexpr (!KEEP) { load_w(i, w); load_pg(g, i, pg); }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float q = b[k] * s1 * (KEEP ? kept_pg[KEEP ? i : 0][k] : pg[k]), e = d[k] * (KEEP ? kept_w[KEEP ? i : 0][k] : w[k]);
+            const float r = q + (p.residual ? p.scale * res[k] : 0.f);
+            if constexpr (V == 1) kept_r[0][k] = r;
+            sum[0] += r * r;
+            sum[1] += e * r;
+            sum[2] += q * (p.grad_new ? dn[k] : 0.f);
+            sum[3] += q * e;
+            sum[4] += q * r;
+          }
+        }
+      }
+      if (ahead && p.post && n + 1 < rows) sum[5] = block_square((n + 1) % p.stages);
+      sums8(sum, slots[n & 1]);
+      const float s2 = rsqrtf(sum[0] * inv_d + p.eps), mean = sum[1] * s2 * inv_d;         // of e xh
+      const float mean_q = (sum[2] + s2 * (sum[3] - s2 * mean * sum[4])) * inv_d;          // of dr q
+      const long long t = t0 + r0 + n;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int v = me + i * tpr;
-        block[i] = dx[i] = none;
-        res[i].zero();
-        dn[i].zero();
         if (v < nvec) {
-          block[i] = *reinterpret_cast<const uint4*>(p.block + t * p.ldb + v * 8);
-          dx[i] = *reinterpret_cast<const uint4*>(p.grad_x + t * p.lddx + v * 8);
-          if (p.residual) res[i].load(p.residual, t * p.ldr + v * 8);
-          if (p.grad_new) dn[i].load(p.grad_new, t * p.lddn + v * 8);
-        }
-      }
-      float s1 = 1.f;
-      if (p.post) {
-        float s[1] = {0.f};
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float b[8];
-          unpack8<ACT>(block[i], b);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) s[0] += b[k] * b[k];
-        }
-        row_reduce<1, false>(s, slots[0], false);
-        s1 = rsqrtf(s[0] * inv_d + p.eps);
-      }
-      float r[V][8], s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float b[8], w[8], q[8];
-        unpack8<ACT>(block[i], b);
-        if (p.post) {
-          unpack8<ACT>(post[i], w);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) b[k] *= s1 * w[k];
-        }
-        if (p.gate) {
-          unpack8<ACT>(gate[i], w);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) b[k] *= w[k];
-        }
-        res[i].get(q);
-        unpack8<ACT>(weight[i], w);
-        float d[8];
-        unpack8<ACT>(dx[i], d);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          r[i][k] = b[k] + p.scale * q[k];
-          s[0] += r[i][k] * r[i][k];
-          s[1] += d[k] * w[k] * r[i][k];
-        }
-      }
-      row_reduce<2, false>(s, slots[1], false);
-      const float s2 = rsqrtf(s[0] * inv_d + p.eps), mean = s[1] * s2 * inv_d;
-      float sf[1] = {0.f};
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int v = me + i * tpr;
-        float b[8], w[8], q[8], d[8], wp[8];
-        unpack8<ACT>(block[i], b);
-        unpack8<ACT>(weight[i], w);
-        unpack8<ACT>(dx[i], d);
-        dn[i].get(q);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float xh = r[i][k] * s2;
-          gw[i][k] += d[k] * xh;
-          q[k] += s2 * (d[k] * w[k] - xh * mean);  // dr
-          w[k] = p.scale * q[k];
-        }
-        if (p.grad_residual && v < nvec) Wide<ACT, F32>::store(p.grad_residual, t * p.lddr + v * 8, w);
-        if (p.post) {
-          unpack8<ACT>(post[i], wp);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) b[k] *= s1;  // bh
-        }
-        if (p.gate) {
-          unpack8<ACT>(gate[i], w);
+          float b[8], d[8], res[8], dn[8], w[8], pg[8], out[8];
+          unpack8<ACT>(lds_u4(at(s, 0, i)), b);
+          unpack8<ACT>(lds_u4(at(s, 1, i)), d);
+          if (V > 1 && p.residual) wide_at(s, 2, i, res);
+          if (p.grad_new) wide_at(s, 2 + WIDE, i, dn);
+          if constexpr (!KEEP) { load_w(i, w); load_pg(g, i, pg); }
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            gg[i][k] += q[k] * (p.post ? b[k] * wp[k] : b[k]);
-            q[k] *= w[k];  // dn
+            const float m = KEEP ? kept_pg[KEEP ? i : 0][k] : pg[k], e = d[k] * (KEEP ? kept_w[KEEP ? i : 0][k] : w[k]);
+            const float bh = b[k] * s1, q = bh * m;
+            const float r = V == 1 ? kept_r[0][k] : q + (p.residual ? p.scale * res[k] : 0.f);
+            const float xh = r * s2;
+            gw[i][k] += d[k] * xh;
+            const float dr = (p.grad_new ? dn[k] : 0.f) + s2 * (e - xh * mean);
+            S[i][k] += dr * bh;
+            res[k] = p.scale * dr;
+            out[k] = p.post ? s1 * (dr * m - bh * mean_q) : dr * m;
           }
+          if (p.grad_residual) Wide<ACT, F32>::store(p.grad_residual, t * p.lddr + v * 8, res);
+          *reinterpret_cast<uint4*>(p.grad_block + t * p.lddb + v * 8) = pack8<ACT>(out);
         }
-        if (p.post) {
+      }
+      s1 = ahead && p.post ? rsqrtf(sum[5] * inv_d + p.eps) : s1;
+    }
+    // the gate's sums: its own gradient, and what the rows give post
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            gp[i][k] += q[k] * b[k];
-            q[k] *= wp[k];  // f
-            sf[0] += q[k] * b[k];
-          }
-        }
+    for (int i = 0; i < V; ++i) {
+      const int v = me + i * tpr;
+      if (v >= nvec) continue;
+      float x[8];
+      if (p.grad_gate) {
+        float* to = p.ctas_per_gate == 1 ? p.grad_gate + (long long)g * p.D : p.partial + ((long long)2 * p.grid + blockIdx.x) * p.D;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) r[i][k] = q[k];
+        for (int k = 0; k < 8; ++k) x[k] = 1.f;
+        if (p.post) unpack8<ACT>(*reinterpret_cast<const uint4*>(p.post + v * 8), x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] *= S[i][k];
+        Wide<ACT, true>::store(to, v * 8, x);
       }
       if (p.post) {
-        row_reduce<1, false>(sf, slots[2], false);
-        const float m = sf[0] * inv_d;
+        const long long to = ((long long)p.grid + blockIdx.x) * p.D + v * 8;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float b[8];
-          unpack8<ACT>(block[i], b);
+        for (int k = 0; k < 8; ++k) x[k] = 1.f;
+        if (p.gate) unpack8<ACT>(*reinterpret_cast<const uint4*>(p.gate + g * p.ldg + v * 8), x);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) r[i][k] = s1 * (r[i][k] - b[k] * s1 * m);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int v = me + i * tpr;
-        if (v < nvec) *reinterpret_cast<uint4*>(p.grad_block + t * p.lddb + v * 8) = pack8<ACT>(r[i]);
-      }
-      if (!p.post) __syncthreads();  // (with one reduction a row its slots are in use until here)
-    }
-    if (p.grad_gate) {
-      float* to = p.ctas_per_gate == 1 ? p.grad_gate + (long long)g * p.D : p.partial + ((long long)2 * p.grid + blockIdx.x) * p.D;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int v = me + i * tpr;
-        if (v < nvec) Wide<ACT, true>::store(to, v * 8, gg[i]);
+        for (int k = 0; k < 8; ++k) x[k] = x[k] * S[i][k] + (first_gate ? 0.f : p.partial[to + k]);
+        Wide<ACT, true>::store(p.partial, to, x);
       }
     }
+    copies_wait(0);  // (what was asked for past the run's end is nothing)
+    __syncthreads();  // the slots of this run's last row have been read
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = me + i * tpr;
-    if (v < nvec) {
-      Wide<ACT, true>::store(p.partial, (long long)blockIdx.x * p.D + v * 8, gw[i]);
-      if (p.post) Wide<ACT, true>::store(p.partial, ((long long)p.grid + blockIdx.x) * p.D + v * 8, gp[i]);
-    }
+    if (v < nvec) Wide<ACT, true>::store(p.partial, (long long)blockIdx.x * p.D + v * 8, gw[i]);
   }
 }
 
@@ -439,6 +517,7 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormBackwardPa
 // grad_post, then one for each gate.
 __global__ void __launch_bounds__(256) norm_sums_kernel(const NormBackwardParams p) {
   __shared__ float part[8][33];
+  start_behind();
   const int which = (int)blockIdx.y, col = (int)blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5;
   const float* from = p.partial;
   float* to = p.grad_weight;
@@ -456,7 +535,7 @@ __global__ void __launch_bounds__(256) norm_sums_kernel(const NormBackwardParams
   float s = 0.f;
   if (col < p.D) {
     const int i0 = n * run / 8, i1 = n * (run + 1) / 8;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = i0; i < i1; ++i) s += from[(long long)i * p.D + col];
   }
   part[run][threadIdx.x & 31] = s;
@@ -470,10 +549,11 @@ __global__ void __launch_bounds__(256) norm_sums_kernel(const NormBackwardParams
 
 // ---- launches ---------------------------------------------------------------------------------------------
 template <class Kernel, class... Args>
-static cudaError_t launch_behind(Kernel kern, dim3 grid, int threads, cudaStream_t stream, const Args&... args) {
+static cudaError_t launch_behind(Kernel kern, dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -508,9 +588,9 @@ static cudaError_t cast_int_act(const CastIntParams& p, cudaStream_t stream) {
   const RowShape s = row_shape(p.T, p.D);
   const dim3 grid((unsigned)s.ctas, 1, 1);
   switch (s.vectors) {
-    case 1: return launch_behind(cast_int_kernel<ACT, 1>, grid, s.threads, stream, p, s.warp_rows);
-    case 2: return launch_behind(cast_int_kernel<ACT, 2>, grid, s.threads, stream, p, s.warp_rows);
-    default: return launch_behind(cast_int_kernel<ACT, 4>, grid, s.threads, stream, p, s.warp_rows);
+    case 1: return launch_behind(cast_int_kernel<ACT, 1>, grid, s.threads, 0, stream, p, s.warp_rows);
+    case 2: return launch_behind(cast_int_kernel<ACT, 2>, grid, s.threads, 0, stream, p, s.warp_rows);
+    default: return launch_behind(cast_int_kernel<ACT, 4>, grid, s.threads, 0, stream, p, s.warp_rows);
   }
 }
 cudaError_t cast_int_launch(const CastIntParams& p, int act, cudaStream_t stream) {
@@ -522,8 +602,8 @@ static cudaError_t norm_type(const NormParams& p, cudaStream_t stream) {
   const RowShape s = row_shape(p.T, p.D);
   const dim3 grid((unsigned)s.ctas, 1, 1);
   switch (s.vectors) {
-    case 1: return launch_behind(norm_kernel<ACT, F32, 1>, grid, s.threads, stream, p, s.warp_rows);
-    default: return launch_behind(norm_kernel<ACT, F32, 2>, grid, s.threads, stream, p, s.warp_rows);
+    case 1: return launch_behind(norm_kernel<ACT, F32, 1>, grid, s.threads, 0, stream, p, s.warp_rows);
+    default: return launch_behind(norm_kernel<ACT, F32, 2>, grid, s.threads, 0, stream, p, s.warp_rows);
   }
 }
 cudaError_t norm_launch(const NormParams& p, int act, bool residual_f32, cudaStream_t stream) {
@@ -531,20 +611,41 @@ cudaError_t norm_launch(const NormParams& p, int act, bool residual_f32, cudaStr
   return residual_f32 ? norm_type<1, true>(p, stream) : norm_type<1, false>(p, stream);
 }
 
+template <int ACT, bool F32, int V>
+static cudaError_t backward_rows(const NormBackwardParams& p, cudaStream_t stream) {
+  static std::atomic<bool> allowed[16];
+  const cudaError_t e = allow_smem(norm_backward_kernel<ACT, F32, V>, allowed);
+  if (e != cudaSuccess) return e;
+  return launch_behind(norm_backward_kernel<ACT, F32, V>, dim3((unsigned)p.grid, 1, 1), p.threads, p.smem, stream, p);
+}
 template <int ACT, bool F32>
 static cudaError_t backward_type(const NormBackwardParams& p, cudaStream_t stream) {
-  const int nvec = p.D / 8, vectors = nvec <= 512 ? 1 : nvec <= 1024 ? 2 : 4;
-  const int threads = ((nvec + vectors - 1) / vectors + 31) / 32 * 32;
-  switch (vectors) {
-    case 1: norm_backward_kernel<ACT, F32, 1><<<p.grid, threads, 0, stream>>>(p); break;
-    case 2: norm_backward_kernel<ACT, F32, 2><<<p.grid, threads, 0, stream>>>(p); break;
-    default: norm_backward_kernel<ACT, F32, 4><<<p.grid, threads, 0, stream>>>(p); break;
+  cudaError_t e;
+  switch (p.vectors) {
+    case 1: e = backward_rows<ACT, F32, 1>(p, stream); break;
+    case 2: e = backward_rows<ACT, F32, 2>(p, stream); break;
+    default: e = backward_rows<ACT, F32, 4>(p, stream); break;
   }
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int sums = 2 + (p.grad_gate && p.ctas_per_gate > 1 ? p.gates : 0);
-  norm_sums_kernel<<<dim3((unsigned)((p.D + 31) / 32), (unsigned)sums, 1), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_behind(norm_sums_kernel, dim3((unsigned)((p.D + 31) / 32), (unsigned)sums, 1), 256, 0, stream, p);
+}
+// The shape of the gradient's launch: threads and vectors of a row, CTAs (one for 512 threads of an SM), and stages for the rows ahead.
+void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gate, int sms, int max_smem, NormBackwardParams* p) {
+  const int nvec = D / 8;
+  p->vectors = nvec <= 512 ? 1 : nvec <= 1024 ? 2 : 4;
+  p->threads = ((nvec + p->vectors - 1) / p->vectors + 31) / 32 * 32;
+  const int per_sm = 512 / p->threads < 4 ? 512 / p->threads : 4, most = sms * per_sm;
+  if (gates >= most) {
+    p->ctas_per_gate = 1;
+    p->grid = most;
+  } else {
+    p->ctas_per_gate = most / gates < tokens_per_gate ? most / gates : tokens_per_gate;
+    p->grid = gates * p->ctas_per_gate;
+  }
+  const int stage = p->vectors * p->threads * 16 * (residual_f32 ? 6 : 4), room = (max_smem + 1024) / per_sm - 1024 - 2048;
+  p->stages = room / stage > 4 ? 4 : room / stage;
+  p->smem = p->stages * stage;
 }
 cudaError_t norm_backward_launch(const NormBackwardParams& p, int act, bool residual_f32, cudaStream_t stream) {
   if (act == 0) return residual_f32 ? backward_type<0, true>(p, stream) : backward_type<0, false>(p, stream);
