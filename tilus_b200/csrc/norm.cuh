@@ -4,6 +4,8 @@
 
 namespace b200q {
 
+constexpr int NORM_BACK_THREADS = 512;  // of an SM in the gradient's kernel, which takes up to 128 registers a thread
+
 struct CastIntParams {
   const unsigned short* x;  // [T, D], row stride ldx, fp16 or bf16
   signed char* out;         // [T, D], row stride ldo

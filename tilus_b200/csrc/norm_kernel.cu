@@ -1,9 +1,10 @@
 // Row-wise kernels between the products of a decoder block: the per-token int8 cast, and the norms before and after a
 // block with its gate and residual scale (norm.cuh has the formulas), forward and backward.
 //
-// All are bound by memory: each input is read once and each output written once, with a row held in registers between the
-// statistics and their use.  Threads own vectors of eight neighbouring channels (16 bytes of a 16-bit type).  Sums and statistics
-// are fp32; the only roundings to fewer bits are those of the outputs.
+// All are bound by memory: each input is read once and each output written once, with a row held on the SM between the
+// statistics and their use.  What keeps them from that bound is the number of instructions, so that threads own several vectors
+// of eight neighbouring channels (16 bytes of a 16-bit type), which share a reduction's steps, and multiply pairs of channels at
+// a time (f32x2).  Sums and statistics are fp32; the only roundings to fewer bits are those of the outputs.
 #include "norm.cuh"
 
 namespace b200q {
@@ -15,84 +16,132 @@ __device__ __forceinline__ void start_behind() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// ---- pairs of fp32 ------------------------------------------------------------------------------------------
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 pair(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 both(float x) { return pair(x, x); }
+__device__ __forceinline__ void split(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float sum(F2 a) {
+  float lo, hi;
+  split(a, lo, hi);
+  return lo + hi;
+}
+
+// eight values of a 16-bit type
 template <int ACT>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const uint4& v, F2 (&f)[4]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (ACT == 0) {
       const float2 t = __half22float2(h2_from_bits(w[i]));
-      f[2 * i] = t.x; f[2 * i + 1] = t.y;
+      f[i] = pair(t.x, t.y);
     } else {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     }
   }
 }
 template <int ACT>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack2<ACT>(f[0], f[1]), pack2<ACT>(f[2], f[3]), pack2<ACT>(f[4], f[5]), pack2<ACT>(f[6], f[7]));
+__device__ __forceinline__ uint4 pack8(const F2 (&f)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    split(f[i], lo, hi);
+    w[i] = pack2<ACT>(lo, hi);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// eight values of the residual stream, of the activation type or fp32
+// eight values of the residual stream, of the activation type or fp32, in one or two 16-byte units
 template <int ACT, bool F32>
 struct Wide {
-  uint4 v[F32 ? 2 : 1];
+  static constexpr int UNITS = F32 ? 2 : 1;
+  uint4 v[UNITS];
   __device__ __forceinline__ void load(const void* base, long long at) {
-    if constexpr (F32) {
-      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + at);
-      v[0] = p[0]; v[1] = p[1];
-    } else {
-      v[0] = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(base) + at);
-    }
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(base) + at * (F32 ? 4 : 2));
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) v[i] = p[i];
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < (F32 ? 2 : 1); ++i) v[i] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < UNITS; ++i) v[i] = make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+  __device__ __forceinline__ void get(F2 (&f)[4]) const {
     if constexpr (F32) {
-      const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+      for (int i = 0; i < 2; ++i) {
+        f[2 * i] = pair(__uint_as_float(v[i].x), __uint_as_float(v[i].y));
+        f[2 * i + 1] = pair(__uint_as_float(v[i].z), __uint_as_float(v[i].w));
+      }
     } else {
       unpack8<ACT>(v[0], f);
     }
   }
-  static __device__ __forceinline__ void store(void* base, long long at, const float (&f)[8]) {
+  static __device__ __forceinline__ void store(void* base, long long at, const F2 (&f)[4]) {
+    uint4* p = reinterpret_cast<uint4*>(static_cast<char*>(base) + at * (F32 ? 4 : 2));
     if constexpr (F32) {
-      float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + at);
-      p[0] = make_float4(f[0], f[1], f[2], f[3]);
-      p[1] = make_float4(f[4], f[5], f[6], f[7]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x[4];
+        split(f[2 * i], x[0], x[1]);
+        split(f[2 * i + 1], x[2], x[3]);
+        p[i] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+      }
     } else {
-      *reinterpret_cast<uint4*>(static_cast<unsigned short*>(base) + at) = pack8<ACT>(f);
+      p[0] = pack8<ACT>(f);
     }
   }
 };
 
-// Sum (or, with MAX, unsigned maximum) of N values over the threads of a row: a warp, or all warps of the CTA.  `slots`: 32 * N words
-// that no other reduction uses until the next barrier but one; every thread gets the same result in the same order.
-template <int N, bool MAX>
-__device__ __forceinline__ void row_reduce(float (&v)[N], float* slots, bool warp_row) {
-  auto join = [](float a, float b) {
-    return MAX ? __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))) : a + b;
-  };
+// ---- reductions over the threads of a row: a warp, or all warps of the CTA -----------------------------------------
+// `slots`: 32 words that no other reduction uses until the next barrier but one; words of warps that the CTA has not are zero.
+// Every thread gets the same result, summed in the same order.
+__device__ __forceinline__ float row_sum(float x, float* slots, bool warp_row) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[i] = join(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
-  if (warp_row) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  if (lane == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) slots[warp * N + i] = v[i];
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if (warp_row) return x;
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = x;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = lane < warps ? slots[lane * N + i] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[i] = join(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
+  x = 0.f;
+  for (int i = 0; i < (int)blockDim.x / 32; i += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(slots + i);
+    x += (s.x + s.y) + (s.z + s.w);
   }
+  return x;
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t x, uint32_t* slots, bool warp_row) {
+  x = __reduce_max_sync(0xffffffffu, x);
+  if (warp_row) return x;
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = 0;
+  for (int i = 0; i < (int)blockDim.x / 32; i += 4) {
+    const uint4 s = *reinterpret_cast<const uint4*>(slots + i);
+    x = max(max(x, max(s.x, s.y)), max(s.z, s.w));
+  }
+  return x;
+}
+// Words of warps that are not there, before the first reduction's barrier.
+template <int N>
+__device__ __forceinline__ void clear_slots(float (&slots)[N][32]) {
+  if (threadIdx.x < 32 && threadIdx.x >= blockDim.x / 32)
+#pragma unroll
+    for (int i = 0; i < N; ++i) slots[i][threadIdx.x] = 0.f;
 }
 
 // ---- per-token int8 cast --------------------------------------------------------------------------------
@@ -105,73 +154,78 @@ __device__ __forceinline__ void int8_scale(float top, float* sf, float* inv) {
   *inv = zero ? 0.0f : __fdiv_rn(127.0f, top);
   if (!(top < __int_as_float(0x7f800000))) *inv = 0.0f;
 }
-// Codes of eight values: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves its low byte in the sum's.
-__device__ __forceinline__ uint2 int8_codes(const float (&f)[8], float inv) {
+// Codes of eight values: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves its low byte in the sum's.  (The
+// product is rounded before: a fused one would see its exact value.)
+__device__ __forceinline__ uint2 int8_codes(const F2 (&f)[4], float inv) {
   uint32_t w[2];
+  const F2 inv2 = both(inv), one = both(1.0f), magic = both(12582912.0f);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[4 * h + i], inv), 12582912.0f));
-    w[h] = inv != 0.0f ? __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) : 0u;
+    float b[4];
+    split(fma2(f[2 * h] * inv2, one, magic), b[0], b[1]);
+    split(fma2(f[2 * h + 1] * inv2, one, magic), b[2], b[3]);
+    w[h] = __byte_perm(__byte_perm(__float_as_uint(b[0]), __float_as_uint(b[1]), 0x0040),
+                       __byte_perm(__float_as_uint(b[2]), __float_as_uint(b[3]), 0x0040), 0x5410);
   }
-  return make_uint2(w[0], w[1]);
+  return inv != 0.0f ? make_uint2(w[0], w[1]) : make_uint2(0, 0);
 }
-// The largest magnitude among 16-bit values, as bits (either type's order like integers, NaN above infinity), two at a time.
-__device__ __forceinline__ uint32_t top_bits(uint32_t top, const uint4& v) {
-  top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
-  return __vmaxu2(__vmaxu2(top, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+// The largest magnitudes of each half of words of two 16-bit values, as bits (NaN wins), and of both as fp32 bits.
+template <int ACT>
+__device__ __forceinline__ uint32_t top2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (ACT == 0) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b & 0x7fff7fffu));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b & 0x7fff7fffu));
+  return r;
 }
 template <int ACT>
-__device__ __forceinline__ float top_value(uint32_t top) {
-  const uint32_t one = max(top & 0xffffu, top >> 16);
-  return ACT == 0 ? __half2float(__ushort_as_half((unsigned short)one)) : __uint_as_float(one << 16);
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, const uint4& v) {
+  return top2<ACT>(top2<ACT>(top2<ACT>(top2<ACT>(top, v.x), v.y), v.z), v.w);
+}
+template <int ACT>
+__device__ __forceinline__ uint32_t top_value(uint32_t top) {
+  const uint32_t one = max(top & 0x7fffu, top >> 16 & 0x7fffu);
+  return ACT == 0 ? __float_as_uint(__half2float(__ushort_as_half((unsigned short)one))) & 0x7fffffffu : one << 16;
 }
 
 template <int ACT, int V>
 __global__ void __launch_bounds__(1024) cast_int_kernel(const CastIntParams p, const int warp_rows) {
-  __shared__ float slots[32];
+  __shared__ __align__(16) float slots[1][32];
   start_behind();
   const bool warp_row = warp_rows != 0;
   const int tpr = warp_row ? 32 : blockDim.x, me = warp_row ? threadIdx.x & 31 : threadIdx.x;
   const int t = warp_row ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   if (t >= p.T) return;  // (whole warps, and only where a warp has its own row)
   const int nvec = p.D / 8;
-  const uint4* row = reinterpret_cast<const uint4*>(p.x + (size_t)t * p.ldx);
+  const uint4* row = reinterpret_cast<const uint4*>(p.x + (size_t)t * p.ldx) + me;
   uint4 keep[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) keep[i] = me + i * tpr < nvec ? row[i * tpr] : make_uint4(0, 0, 0, 0);
+  clear_slots(slots);
   uint32_t bits = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int v = me + i * tpr;
-    keep[i] = v < nvec ? row[v] : make_uint4(0, 0, 0, 0);
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) bits = top_bits(bits, keep[i]);
-  for (int v = me + V * tpr; v < nvec; v += tpr) bits = top_bits(bits, row[v]);  // (what does not stay in registers is read again)
-  float top[1] = {top_value<ACT>(bits)};
-  row_reduce<1, true>(top, slots, warp_row);
+  for (int i = 0; i < V; ++i) bits = top_bits<ACT>(bits, keep[i]);
+  for (int i = V; me + i * tpr < nvec; ++i) bits = top_bits<ACT>(bits, row[i * tpr]);  // (what does not stay in registers is read again)
   float sf, inv;
-  int8_scale(top[0], &sf, &inv);
+  int8_scale(__uint_as_float(row_max(top_value<ACT>(bits), reinterpret_cast<uint32_t*>(slots[0]), warp_row)), &sf, &inv);
   if (me == 0) p.out_sf[t] = sf;
-  uint2* out = reinterpret_cast<uint2*>(p.out + (size_t)t * p.ldo);
+  uint2* out = reinterpret_cast<uint2*>(p.out + (size_t)t * p.ldo) + me;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int v = me + i * tpr;
-    float f[8];
+    F2 f[4];
     unpack8<ACT>(keep[i], f);
-    if (v < nvec) out[v] = int8_codes(f, inv);
+    if (me + i * tpr < nvec) out[i * tpr] = int8_codes(f, inv);
   }
-  for (int v = me + V * tpr; v < nvec; v += tpr) {
-    float f[8];
-    unpack8<ACT>(row[v], f);
-    out[v] = int8_codes(f, inv);
+  for (int i = V; me + i * tpr < nvec; ++i) {
+    F2 f[4];
+    unpack8<ACT>(row[i * tpr], f);
+    out[i * tpr] = int8_codes(f, inv);
   }
 }
 
 // ---- block norm -------------------------------------------------------------------------------------------
 template <int ACT, bool F32, int V>
-__global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const int warp_rows) {
-  __shared__ float slots[3][32];
+__global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_kernel(const NormParams p, const int warp_rows) {
+  __shared__ __align__(16) float slots[3][32];
   start_behind();
   const bool warp_row = warp_rows != 0;
   const int tpr = warp_row ? 32 : blockDim.x, me = warp_row ? threadIdx.x & 31 : threadIdx.x;
@@ -179,82 +233,94 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const in
   if (t >= p.T) return;
   const int nvec = p.D / 8;
   const float inv_d = 1.0f / (float)p.D;
-  float r[V][8];  // block, then the new residual, then x
+  const uint4 none = make_uint4(0, 0, 0, 0);
+  F2 r[V][4];  // block, then the new residual, then x
   Wide<ACT, F32> res[V];
+  uint4 raw[V], ahead[V][2];  // one vector or two: the weights of what comes first are asked for with the row
+  const unsigned short* gate = p.gate ? p.gate + (t / p.tokens_per_gate) * p.ldg : nullptr;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = me + i * tpr;
-    uint4 b = make_uint4(0, 0, 0, 0);
+    raw[i] = none;
     res[i].zero();
     if (v < nvec) {
-      b = *reinterpret_cast<const uint4*>(p.block + t * p.ldb + v * 8);
+      raw[i] = *reinterpret_cast<const uint4*>(p.block + t * p.ldb + v * 8);
       if (p.residual) res[i].load(p.residual, t * p.ldr + v * 8);
     }
-    unpack8<ACT>(b, r[i]);
   }
+  auto weights = [&](const unsigned short* from, int v) { return v < nvec ? *reinterpret_cast<const uint4*>(from + v * 8) : none; };
+  if constexpr (V <= 2) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (p.post) ahead[i][0] = weights(p.post, me + i * tpr);
+      if (gate) ahead[i][1] = weights(gate, me + i * tpr);
+    }
+  }
+  clear_slots(slots);
+#pragma unroll
+  for (int i = 0; i < V; ++i) unpack8<ACT>(raw[i], r[i]);
+  const F2 zero = both(0.f);
   if (p.post) {
-    float s[1] = {0.f};
+    F2 s = zero;
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[0] += r[i][k] * r[i][k];
-    row_reduce<1, false>(s, slots[0], warp_row);
-    const float inv = rsqrtf(s[0] * inv_d + p.eps);
+      for (int k = 0; k < 4; ++k) s = fma2(r[i][k], r[i][k], s);
+    const F2 inv = both(rsqrtf(row_sum(sum(s), slots[0], warp_row) * inv_d + p.eps));
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int v = me + i * tpr;
-      if (v < nvec) {
-        float w[8];
-        unpack8<ACT>(*reinterpret_cast<const uint4*>(p.post + v * 8), w);
+      F2 w[4];
+      unpack8<ACT>(V <= 2 ? ahead[i][0] : weights(p.post, me + i * tpr), w);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) r[i][k] *= inv * w[k];
-      }
+      for (int k = 0; k < 4; ++k) r[i][k] = r[i][k] * (inv * w[k]);
     }
   }
-  const unsigned short* gate = p.gate ? p.gate + (t / p.tokens_per_gate) * p.ldg : nullptr;
-  float s[1] = {0.f};
+  if (gate) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      F2 w[4];
+      unpack8<ACT>(V <= 2 ? ahead[i][1] : weights(gate, me + i * tpr), w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[i][k] = r[i][k] * w[k];
+    }
+  }
+  F2 s = zero;
+  const F2 scale = both(p.scale);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = me + i * tpr;
-    float q[8];
-    if (gate && v < nvec) {
-      unpack8<ACT>(*reinterpret_cast<const uint4*>(gate + v * 8), q);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r[i][k] *= q[k];
-    }
+    F2 q[4];
     res[i].get(q);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      r[i][k] += p.scale * q[k];
-      s[0] += r[i][k] * r[i][k];
+    for (int k = 0; k < 4; ++k) {
+      r[i][k] = fma2(scale, q[k], r[i][k]);
+      s = fma2(r[i][k], r[i][k], s);
     }
     if (v < nvec) Wide<ACT, F32>::store(p.new_residual, t * p.ldn + v * 8, r[i]);
   }
-  row_reduce<1, false>(s, slots[1], warp_row);
-  const float inv = rsqrtf(s[0] * inv_d + p.eps);
+  if constexpr (V <= 2)
+#pragma unroll
+    for (int i = 0; i < V; ++i) ahead[i][0] = weights(p.weight, me + i * tpr);
+  const F2 inv = both(rsqrtf(row_sum(sum(s), slots[1], warp_row) * inv_d + p.eps));
   uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = me + i * tpr;
-    if (v < nvec) {
-      float w[8];
-      unpack8<ACT>(*reinterpret_cast<const uint4*>(p.weight + v * 8), w);
+    F2 w[4];
+    unpack8<ACT>(V <= 2 ? ahead[i][0] : weights(p.weight, v), w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) r[i][k] *= inv * w[k];
-      const uint4 x = pack8<ACT>(r[i]);
-      if (p.x) {
-        *reinterpret_cast<uint4*>(p.x + t * p.ldx + v * 8) = x;
-      } else {
-        unpack8<ACT>(x, r[i]);  // what is cast is the rounded x: the codes are those of a cast of it
-        bits = top_bits(bits, x);
-      }
+    for (int k = 0; k < 4; ++k) r[i][k] = r[i][k] * (inv * w[k]);
+    const uint4 x = pack8<ACT>(r[i]);
+    if (p.x) {
+      if (v < nvec) *reinterpret_cast<uint4*>(p.x + t * p.ldx + v * 8) = x;
+    } else {
+      unpack8<ACT>(x, r[i]);  // what is cast is the rounded x: the codes are those of a cast of it
+      if (v < nvec) bits = top_bits<ACT>(bits, x);
     }
   }
   if (!p.x) {
-    float top[1] = {top_value<ACT>(bits)};
-    row_reduce<1, true>(top, slots[2], warp_row);
     float sf, qinv;
-    int8_scale(top[0], &sf, &qinv);
+    int8_scale(__uint_as_float(row_max(top_value<ACT>(bits), reinterpret_cast<uint32_t*>(slots[2]), warp_row)), &sf, &qinv);
     if (me == 0) p.x_sf[t] = sf;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -311,52 +377,46 @@ __device__ __forceinline__ void sums8(float (&v)[8], float* slots) {
   x += __shfl_xor_sync(0xffffffffu, x, 8);
   x += __shfl_xor_sync(0xffffffffu, x, 16);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __shfl_sync(0xffffffffu, x, i);
+  for (int i = 0; i < 6; ++i) v[i] = __shfl_sync(0xffffffffu, x, i);
 }
 
 // V: vectors of eight channels to a thread.  Up to two, the weights of a thread's channels stay in registers too.
 template <int ACT, bool F32, int V>
-__global__ void __launch_bounds__(512) norm_backward_kernel(const NormBackwardParams p) {
+__global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const NormBackwardParams p) {
   extern __shared__ __align__(16) unsigned char rows_smem[];
-  __shared__ float slots[2][128], slots_block[512 / 32];
+  __shared__ __align__(16) float slots[2][8 * (NORM_BACK_THREADS / 32)], slots_block[1][32];
   constexpr int WIDE = F32 ? 2 : 1, UNITS = 2 + 2 * WIDE;  // 16-byte units of a vector: block, grad_x, residual, grad_new
   constexpr bool KEEP = V <= 2;
   start_behind();
+  clear_slots(slots_block);
   const int me = threadIdx.x, tpr = blockDim.x, nvec = p.D / 8;
   const float inv_d = 1.0f / (float)p.D;
-  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(rows_smem) + (uint32_t)me * 16u;
-  // the unit u of vector i in stage s
-  auto at = [&](int s, int u, int i) { return mine + (uint32_t)(((s * UNITS + u) * V + i) * tpr) * 16u; };
-  auto wide_at = [&](int s, int u, int i, float (&f)[8]) {
-    Wide<ACT, F32> w;
-#pragma unroll
-    for (int h = 0; h < WIDE; ++h) w.v[h] = lds_u4(at(s, u + h, i));
-    w.get(f);
-  };
-  // The weights of a vector's channels: of the second norm, and of what stands in front of the residual (post and gate together)
-  auto load_w = [&](int i, float (&w)[8]) {
+  const F2 zero = both(0.f), scale = both(p.scale);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rows_smem) + (uint32_t)me * 16u;
+  const uint32_t unit = (uint32_t)tpr * 16u, stage = unit * (UNITS * V), ring_end = ring + stage * (uint32_t)p.stages;
+  auto at = [&](uint32_t s, int u, int i) { return s + unit * (uint32_t)(u * V + i); };  // unit u of vector i in the stage at s
+  auto load = [&](const unsigned short* from, int i, F2 (&w)[4]) {
     const int v = me + i * tpr;
-    unpack8<ACT>(v < nvec ? *reinterpret_cast<const uint4*>(p.weight + v * 8) : make_uint4(0, 0, 0, 0), w);
+    unpack8<ACT>(v < nvec ? *reinterpret_cast<const uint4*>(from + v * 8) : make_uint4(0, 0, 0, 0), w);
   };
-  auto load_pg = [&](int g, int i, float (&pg)[8]) {
-    const int v = me + i * tpr;
+  // what stands in front of a row's block in the new residual: post and gate together
+  auto load_pg = [&](int g, int i, F2 (&pg)[4]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) pg[k] = 1.f;
-    float x[8];
-    if (p.post && v < nvec) unpack8<ACT>(*reinterpret_cast<const uint4*>(p.post + v * 8), pg);
-    if (p.gate && v < nvec) {
-      unpack8<ACT>(*reinterpret_cast<const uint4*>(p.gate + g * p.ldg + v * 8), x);
+    for (int k = 0; k < 4; ++k) pg[k] = both(1.f);
+    if (p.post) load(p.post, i, pg);
+    if (p.gate) {
+      F2 x[4];
+      load(p.gate + g * p.ldg, i, x);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) pg[k] *= x[k];
+      for (int k = 0; k < 4; ++k) pg[k] = pg[k] * x[k];
     }
   };
-  float kept_w[KEEP ? V : 1][8], kept_pg[KEEP ? V : 1][8];
-  float gw[V][8], S[V][8];
+  F2 kept_w[KEEP ? V : 1][4], kept_pg[KEEP ? V : 1][4], gw[V][4], S[V][4];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    if constexpr (KEEP) load_w(i, kept_w[i]);
+    if constexpr (KEEP) load(p.weight, i, kept_w[i]);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) gw[i][k] = 0.f;
+    for (int k = 0; k < 4; ++k) gw[i][k] = zero;
   }
   // Three stages and more: a row's reduction takes the next row's sum of block block along, whose copies have landed by then.
   const bool ahead = p.stages >= 3;
@@ -367,143 +427,160 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormBackwardPa
     for (int i = 0; i < V; ++i) {
       if constexpr (KEEP) load_pg(g, i, kept_pg[i]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) S[i][k] = 0.f;
+      for (int k = 0; k < 4; ++k) S[i][k] = zero;
     }
-    const long long t0 = (long long)g * p.tokens_per_gate;
     const int r0 = (int)((long long)p.tokens_per_gate * part / p.ctas_per_gate);
     const int rows = (int)((long long)p.tokens_per_gate * (part + 1) / p.ctas_per_gate) - r0;
-    auto fetch = [&](int n) {  // row n of this run, to stage n % stages
-      if (n < rows) {
-        const long long t = t0 + r0 + n;
-        const int s = n % p.stages;
+    // this thread's first vector of the next row to be copied and of the next to be written
+    const long long t0 = (long long)g * p.tokens_per_gate + r0;
+    const char* from_b = reinterpret_cast<const char*>(p.block + t0 * p.ldb) + me * 16;
+    const char* from_x = reinterpret_cast<const char*>(p.grad_x + t0 * p.lddx) + me * 16;
+    const char* from_r = static_cast<const char*>(p.residual) + (t0 * p.ldr + me * 8) * (F32 ? 4 : 2);
+    const char* from_n = static_cast<const char*>(p.grad_new) + (t0 * p.lddn + me * 8) * (F32 ? 4 : 2);
+    long long to_b = t0 * p.lddb + me * 8, to_r = t0 * p.lddr + me * 8;
+    int asked = 0;
+    uint32_t ask_at = ring;
+    auto fetch = [&]() {  // the next row of this run, to the next stage
+      if (asked < rows) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const int v = me + i * tpr;
-          if (v < nvec) {
-            copy16(at(s, 0, i), p.block + t * p.ldb + v * 8);
-            copy16(at(s, 1, i), p.grad_x + t * p.lddx + v * 8);
+          if (me + i * tpr < nvec) {
+            copy16(at(ask_at, 0, i), from_b + i * unit);
+            copy16(at(ask_at, 1, i), from_x + i * unit);
 #pragma unroll
             for (int h = 0; h < WIDE; ++h) {
-              if (p.residual) copy16(at(s, 2 + h, i), static_cast<const char*>(p.residual) + (t * p.ldr + v * 8) * (F32 ? 4 : 2) + h * 16);
-              if (p.grad_new) copy16(at(s, 2 + WIDE + h, i), static_cast<const char*>(p.grad_new) + (t * p.lddn + v * 8) * (F32 ? 4 : 2) + h * 16);
+              if (p.residual) copy16(at(ask_at, 2 + h, i), from_r + i * unit * WIDE + h * 16);
+              if (p.grad_new) copy16(at(ask_at, 2 + WIDE + h, i), from_n + i * unit * WIDE + h * 16);
             }
           }
         }
+        from_b += p.ldb * 2; from_x += p.lddx * 2;
+        from_r += p.ldr * (F32 ? 4 : 2); from_n += p.lddn * (F32 ? 4 : 2);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
+      ++asked;
+      ask_at = ask_at + stage == ring_end ? ring : ask_at + stage;
     };
-    auto block_square = [&](int s) {
-      float x = 0.f;
+    auto block_square = [&](uint32_t s) {
+      F2 x = zero;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float b[8];
-        unpack8<ACT>(lds_u4(at(s, 0, i)), b);
-        if (me + i * tpr < nvec)
+      for (int i = 0; i < V; ++i)
+        if (me + i * tpr < nvec) {
+          F2 b[4];
+          unpack8<ACT>(lds_u4(at(s, 0, i)), b);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x += b[k] * b[k];
-      }
-      return x;
+          for (int k = 0; k < 4; ++k) x = fma2(b[k], b[k], x);
+        }
+      return sum(x);
     };
-    for (int n = 0; n < p.stages - 1; ++n) fetch(n);
+    auto wide = [&](const void* there, uint32_t s, int u, int i, F2 (&f)[4]) {
+      Wide<ACT, F32> w;
+      w.zero();
+      if (there)
+#pragma unroll
+        for (int h = 0; h < WIDE; ++h) w.v[h] = lds_u4(at(s, u + h, i));
+      w.get(f);
+    };
+    for (int n = 0; n < p.stages - 1; ++n) fetch();
     float s1 = 1.f;
     if (ahead && p.post && rows > 0) {
       copies_wait(p.stages - 2);
-      float x[1] = {block_square(0)};
-      row_reduce<1, false>(x, slots_block, false);
-      s1 = rsqrtf(x[0] * inv_d + p.eps);
+      s1 = rsqrtf(row_sum(block_square(ring), slots_block[0], false) * inv_d + p.eps);
     }
+    uint32_t s = ring;
     for (int n = 0; n < rows; ++n) {
-      const int s = n % p.stages;
-      fetch(n + p.stages - 1);
+      const uint32_t next = s + stage == ring_end ? ring : s + stage;
+      fetch();
       copies_wait(ahead ? p.stages - 2 : p.stages - 1);
-      if (!ahead && p.post) {
-        float x[1] = {block_square(s)};
-        row_reduce<1, false>(x, slots_block, false);
-        s1 = rsqrtf(x[0] * inv_d + p.eps);
-      }
-      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      float kept_r[1][8];
+      if (!ahead && p.post) s1 = rsqrtf(row_sum(block_square(s), slots_block[0], false) * inv_d + p.eps);
+      F2 rr = zero, er = zero, qn = zero, qe = zero, qr = zero;
+      const F2 s1_2 = both(s1);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         if (me + i * tpr < nvec) {
-          float b[8], d[8], res[8], dn[8], w[8], pg[8];
+          F2 b[4], d[4], res[4], dn[4], w[4], pg[4];
           unpack8<ACT>(lds_u4(at(s, 0, i)), b);
           unpack8<ACT>(lds_u4(at(s, 1, i)), d);
-          if (p.residual) wide_at(s, 2, i, res);
-          if (p.grad_new) wide_at(s, 2 + WIDE, i, dn);
-          if constexpr (!KEEP) { load_w(i, w); load_pg(g, i, pg); }
+          wide(p.residual, s, 2, i, res);
+          wide(p.grad_new, s, 2 + WIDE, i, dn);
+          if constexpr (!KEEP) { load(p.weight, i, w); load_pg(g, i, pg); }
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float q = b[k] * s1 * (KEEP ? kept_pg[KEEP ? i : 0][k] : pg[k]), e = d[k] * (KEEP ? kept_w[KEEP ? i : 0][k] : w[k]);
-            const float r = q + (p.residual ? p.scale * res[k] : 0.f);
-            if constexpr (V == 1) kept_r[0][k] = r;
-            sum[0] += r * r;
-            sum[1] += e * r;
-            sum[2] += q * (p.grad_new ? dn[k] : 0.f);
-            sum[3] += q * e;
-            sum[4] += q * r;
+          for (int k = 0; k < 4; ++k) {
+            const F2 q = (b[k] * s1_2) * (KEEP ? kept_pg[KEEP ? i : 0][k] : pg[k]), e = d[k] * (KEEP ? kept_w[KEEP ? i : 0][k] : w[k]);
+            const F2 r = fma2(scale, res[k], q);
+            rr = fma2(r, r, rr);
+            er = fma2(e, r, er);
+            qn = fma2(q, dn[k], qn);
+            qe = fma2(q, e, qe);
+            qr = fma2(q, r, qr);
           }
         }
       }
-      if (ahead && p.post && n + 1 < rows) sum[5] = block_square((n + 1) % p.stages);
-      sums8(sum, slots[n & 1]);
-      const float s2 = rsqrtf(sum[0] * inv_d + p.eps), mean = sum[1] * s2 * inv_d;         // of e xh
-      const float mean_q = (sum[2] + s2 * (sum[3] - s2 * mean * sum[4])) * inv_d;          // of dr q
-      const long long t = t0 + r0 + n;
+      float x[8] = {sum(rr), sum(er), sum(qn), sum(qe), sum(qr), 0.f, 0.f, 0.f};
+      if (ahead && p.post && n + 1 < rows) x[5] = block_square(next);
+      sums8(x, slots[n & 1]);
+      const float s2 = rsqrtf(x[0] * inv_d + p.eps), mean = x[1] * s2 * inv_d;                       // of e xh
+      const float mean_q = p.post ? (x[2] + s2 * (x[3] - s2 * mean * x[4])) * inv_d : 0.f;           // of dr q
+      const F2 s2_2 = both(s2), mean_2 = both(-mean), mean_q2 = both(-mean_q);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int v = me + i * tpr;
         if (v < nvec) {
-          float b[8], d[8], res[8], dn[8], w[8], pg[8], out[8];
+          F2 b[4], d[4], res[4], dn[4], w[4], pg[4], out[4];
           unpack8<ACT>(lds_u4(at(s, 0, i)), b);
           unpack8<ACT>(lds_u4(at(s, 1, i)), d);
-          if (V > 1 && p.residual) wide_at(s, 2, i, res);
-          if (p.grad_new) wide_at(s, 2 + WIDE, i, dn);
-          if constexpr (!KEEP) { load_w(i, w); load_pg(g, i, pg); }
+          wide(p.residual, s, 2, i, res);
+          wide(p.grad_new, s, 2 + WIDE, i, dn);
+          if constexpr (!KEEP) { load(p.weight, i, w); load_pg(g, i, pg); }
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float m = KEEP ? kept_pg[KEEP ? i : 0][k] : pg[k], e = d[k] * (KEEP ? kept_w[KEEP ? i : 0][k] : w[k]);
-            const float bh = b[k] * s1, q = bh * m;
-            const float r = V == 1 ? kept_r[0][k] : q + (p.residual ? p.scale * res[k] : 0.f);
-            const float xh = r * s2;
-            gw[i][k] += d[k] * xh;
-            const float dr = (p.grad_new ? dn[k] : 0.f) + s2 * (e - xh * mean);
-            S[i][k] += dr * bh;
-            res[k] = p.scale * dr;
-            out[k] = p.post ? s1 * (dr * m - bh * mean_q) : dr * m;
+          for (int k = 0; k < 4; ++k) {
+            const F2 m = KEEP ? kept_pg[KEEP ? i : 0][k] : pg[k];
+            const F2 bh = b[k] * s1_2, xh = fma2(scale, res[k], bh * m) * s2_2;
+            gw[i][k] = fma2(d[k], xh, gw[i][k]);
+            const F2 dr = fma2(s2_2, fma2(mean_2, xh, d[k] * (KEEP ? kept_w[KEEP ? i : 0][k] : w[k])), dn[k]);
+            S[i][k] = fma2(dr, bh, S[i][k]);
+            res[k] = scale * dr;
+            out[k] = s1_2 * fma2(mean_q2, bh, dr * m);
           }
-          if (p.grad_residual) Wide<ACT, F32>::store(p.grad_residual, t * p.lddr + v * 8, res);
-          *reinterpret_cast<uint4*>(p.grad_block + t * p.lddb + v * 8) = pack8<ACT>(out);
+          if (p.grad_residual) Wide<ACT, F32>::store(p.grad_residual, to_r + i * tpr * 8, res);
+          *reinterpret_cast<uint4*>(p.grad_block + to_b + i * tpr * 8) = pack8<ACT>(out);
         }
       }
-      s1 = ahead && p.post ? rsqrtf(sum[5] * inv_d + p.eps) : s1;
+      to_b += p.lddb; to_r += p.lddr;
+      if (ahead && p.post) s1 = rsqrtf(x[5] * inv_d + p.eps);
+      s = next;
     }
-    // the gate's sums: its own gradient, and what the rows give post
+    // the gate's sums: its own gradient, and what its rows give post
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int v = me + i * tpr;
       if (v >= nvec) continue;
-      float x[8];
+      F2 x[4];
       if (p.grad_gate) {
         float* to = p.ctas_per_gate == 1 ? p.grad_gate + (long long)g * p.D : p.partial + ((long long)2 * p.grid + blockIdx.x) * p.D;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = 1.f;
-        if (p.post) unpack8<ACT>(*reinterpret_cast<const uint4*>(p.post + v * 8), x);
+        for (int k = 0; k < 4; ++k) x[k] = both(1.f);
+        if (p.post) load(p.post, i, x);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] *= S[i][k];
+        for (int k = 0; k < 4; ++k) x[k] = x[k] * S[i][k];
         Wide<ACT, true>::store(to, v * 8, x);
       }
       if (p.post) {
         const long long to = ((long long)p.grid + blockIdx.x) * p.D + v * 8;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = 1.f;
-        if (p.gate) unpack8<ACT>(*reinterpret_cast<const uint4*>(p.gate + g * p.ldg + v * 8), x);
+        for (int k = 0; k < 4; ++k) x[k] = both(1.f);
+        if (p.gate) load(p.gate + g * p.ldg, i, x);
+        Wide<ACT, true> sofar;
+        F2 y[4];
+        sofar.zero();
+        if (!first_gate) sofar.load(p.partial, to);
+        sofar.get(y);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = x[k] * S[i][k] + (first_gate ? 0.f : p.partial[to + k]);
+        for (int k = 0; k < 4; ++k) x[k] = fma2(x[k], S[i][k], y[k]);
         Wide<ACT, true>::store(p.partial, to, x);
       }
     }
-    copies_wait(0);  // (what was asked for past the run's end is nothing)
+    copies_wait(0);   // (what was asked for past the run's end is nothing)
     __syncthreads();  // the slots of this run's last row have been read
   }
 #pragma unroll
@@ -563,9 +640,10 @@ static cudaError_t launch_behind(Kernel kern, dim3 grid, int threads, int smem, 
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// Threads of a row and vectors of a thread: a warp for up to 512 channels, else a CTA.
+// Threads of a row and vectors of a thread: a warp for up to 512 channels, else a CTA.  Where rows are many, 256 threads with up to
+// eight vectors, so that the steps of a reduction are shared by many channels; where they are few, as many as the row has.
 struct RowShape { int warp_rows, threads, vectors, ctas; };
-static RowShape row_shape(int T, int D) {
+static RowShape row_shape(int T, int D, int most_vectors) {
   const int nvec = D / 8;
   RowShape s;
   s.warp_rows = nvec <= 64 ? 1 : 0;
@@ -575,22 +653,25 @@ static RowShape row_shape(int T, int D) {
     s.ctas = (T + 3) / 4;
     return s;
   }
-  s.vectors = nvec <= 256 ? 1 : nvec <= 2048 ? 2 : 4;
+  const int threads = T <= 296 ? 512 : 256;
+  s.vectors = 1;
+  while (s.vectors < most_vectors && s.vectors * threads < nvec) s.vectors *= 2;
   const int per = (nvec + s.vectors - 1) / s.vectors;
   s.threads = (per + 31) / 32 * 32;
-  if (s.threads > 1024) s.threads = 1024;
+  if (s.threads > 512) s.threads = 512;
   s.ctas = T;
   return s;
 }
 
 template <int ACT>
 static cudaError_t cast_int_act(const CastIntParams& p, cudaStream_t stream) {
-  const RowShape s = row_shape(p.T, p.D);
+  const RowShape s = row_shape(p.T, p.D, 8);
   const dim3 grid((unsigned)s.ctas, 1, 1);
   switch (s.vectors) {
     case 1: return launch_behind(cast_int_kernel<ACT, 1>, grid, s.threads, 0, stream, p, s.warp_rows);
     case 2: return launch_behind(cast_int_kernel<ACT, 2>, grid, s.threads, 0, stream, p, s.warp_rows);
-    default: return launch_behind(cast_int_kernel<ACT, 4>, grid, s.threads, 0, stream, p, s.warp_rows);
+    case 4: return launch_behind(cast_int_kernel<ACT, 4>, grid, s.threads, 0, stream, p, s.warp_rows);
+    default: return launch_behind(cast_int_kernel<ACT, 8>, grid, s.threads, 0, stream, p, s.warp_rows);
   }
 }
 cudaError_t cast_int_launch(const CastIntParams& p, int act, cudaStream_t stream) {
@@ -599,11 +680,13 @@ cudaError_t cast_int_launch(const CastIntParams& p, int act, cudaStream_t stream
 
 template <int ACT, bool F32>
 static cudaError_t norm_type(const NormParams& p, cudaStream_t stream) {
-  const RowShape s = row_shape(p.T, p.D);
+  const RowShape s = row_shape(p.T, p.D, 8);
   const dim3 grid((unsigned)s.ctas, 1, 1);
   switch (s.vectors) {
     case 1: return launch_behind(norm_kernel<ACT, F32, 1>, grid, s.threads, 0, stream, p, s.warp_rows);
-    default: return launch_behind(norm_kernel<ACT, F32, 2>, grid, s.threads, 0, stream, p, s.warp_rows);
+    case 2: return launch_behind(norm_kernel<ACT, F32, 2>, grid, s.threads, 0, stream, p, s.warp_rows);
+    case 4: return launch_behind(norm_kernel<ACT, F32, 4>, grid, s.threads, 0, stream, p, s.warp_rows);
+    default: return launch_behind(norm_kernel<ACT, F32, 8>, grid, s.threads, 0, stream, p, s.warp_rows);
   }
 }
 cudaError_t norm_launch(const NormParams& p, int act, bool residual_f32, cudaStream_t stream) {
@@ -630,12 +713,12 @@ static cudaError_t backward_type(const NormBackwardParams& p, cudaStream_t strea
   const int sums = 2 + (p.grad_gate && p.ctas_per_gate > 1 ? p.gates : 0);
   return launch_behind(norm_sums_kernel, dim3((unsigned)((p.D + 31) / 32), (unsigned)sums, 1), 256, 0, stream, p);
 }
-// The shape of the gradient's launch: threads and vectors of a row, CTAs (one for 512 threads of an SM), and stages for the rows ahead.
+// The shape of the gradient's launch: threads and vectors of a row, CTAs (512 threads to an SM), and stages for the rows ahead.
 void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gate, int sms, int max_smem, NormBackwardParams* p) {
   const int nvec = D / 8;
-  p->vectors = nvec <= 512 ? 1 : nvec <= 1024 ? 2 : 4;
+  p->vectors = nvec <= 256 ? 1 : nvec <= 1024 ? 2 : 4;
   p->threads = ((nvec + p->vectors - 1) / p->vectors + 31) / 32 * 32;
-  const int per_sm = 512 / p->threads < 4 ? 512 / p->threads : 4, most = sms * per_sm;
+  const int per_sm = NORM_BACK_THREADS / p->threads < 4 ? NORM_BACK_THREADS / p->threads : 4, most = sms * per_sm;
   if (gates >= most) {
     p->ctas_per_gate = 1;
     p->grid = most;
