@@ -361,8 +361,8 @@ int b200q_igemm_planned(const void* a, int lda, const void* b, int ldb, const fl
  * b200q_block_norm_backward: from grad_x (act_dtype) and grad_new (of r', its type; NULL: zero) the gradients of block
  * (act_dtype), residual (its type; NULL: not wanted), and in fp32 of weight [hidden], post_weight [hidden] and gate
  * [gates, hidden] (given exactly where the operand is).  What the forward pass computed is computed again from its inputs.
- * `scratch`: b200q_block_norm_scratch_bytes(...) bytes of this call's own, need not be cleared.  The same inputs give the
- * same bits. */
+ * `scratch`: b200q_block_norm_scratch_bytes(...) bytes of this call's own, need not be cleared; `workspace` holds the
+ * status header (256 bytes).  The same inputs give the same bits. */
 typedef struct b200q_block_norm {
   const void *block, *residual, *weight, *post_weight, *gate;
   int64_t ldb, ldr, ldg;  /* row strides of block, residual, gate */
@@ -377,14 +377,14 @@ size_t b200q_block_norm_scratch_bytes(int tokens, int hidden, int gates);
 int b200q_block_norm_backward(const b200q_block_norm_t* args, const void* grad_x, long long lddx, const void* grad_new,
                               long long lddn, void* grad_block, long long lddb, void* grad_residual, long long lddr,
                               float* grad_weight, float* grad_post, float* grad_gate, void* scratch, size_t scratch_bytes,
-                              void* stream);
+                              void* workspace, size_t workspace_bytes, void* stream);
 
 /* Reads the device status header of a workspace (synchronises `stream`): status[0] is 0 or
  * B200Q_ERR_DEVICE_TIMEOUT, status[1..3] say which wait gave up (1: 2 = tcgen05 prefill pipeline,
  * 3 = stream kernel's weight ring, 5 = wait for a peer's columns, 6 = tcgen05 small-batch pipeline,
  * 7 / 8 = gather push / collect, 9 = wait for the CTAs that fetch host activations, 10 = exact
  * small-batch kernel's pipeline, 11 = a wait of the kernel that keeps the activations in registers, 12 = pair kernel of
- * the 8-bit products, 13 = their stream kernel; 2: CTA; 3: warp or thread).  Clears the header.  A launch that gave up may leave partial sums
+ * the 8-bit products, 13 = their stream kernel, 14 = the gradient of the block norm; 2: CTA; 3: warp or thread).  Clears the header.  A launch that gave up may leave partial sums
  * behind: zero the workspace before it is used again.  workspace == NULL names the built-in
  * scratch of b200q_gemm_static_ws, which this call then puts back to zero itself. */
 int b200q_device_status(void* workspace, int32_t status[4], void* stream);

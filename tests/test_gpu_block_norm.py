@@ -55,7 +55,7 @@ def _close(got, want, size, roundings=128):
     assert bool((err <= bound).all()), float((err / bound.clamp(min=1e-300)).max())
 
 
-CASES = [(1, 8), (1, 4096), (3, 264), (5, 512), (7, 520), (2, 1000), (130, 2048), (33, 4104), (64, 5120), (3, 8192), (2, 8200), (6, 16384)]
+CASES = [(1, 8), (1, 4096), (3, 264), (5, 512), (7, 520), (2, 1000), (130, 2048), (1030, 520), (1030, 1032), (1100, 2056), (900, 4096), (33, 4104), (64, 5120), (3, 8192), (2, 8200), (6, 16384)]
 FORMS = [dict(), dict(post=True, gates=1), dict(wide=True, gates=1), dict(wide=True, post=True), dict(residual=False, post=True)]
 
 

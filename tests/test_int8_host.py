@@ -80,10 +80,10 @@ def test_bad_norms_are_refused_before_a_launch(lib):
         assert lib.b200q_block_norm(_norm(), x, ldx, codes, sf, new, 64, None) == 1
     assert lib.b200q_block_norm(None, ok, 64, None, None, ok, 64, None) == 1
     good = dict(args=_norm(), dx=ok, lddx=64, dn=None, lddn=0, db=ok, lddb=64, dr=ok, lddr=64, dw=ok, dp=None, dg=None, s=ok,
-                n=1 << 30, stream=None)
+                n=1 << 30, ws=ok, ws_bytes=256, stream=None)
     for bad, status in ((dict(dx=None), 1), (dict(db=None), 1), (dict(dw=None), 1), (dict(dp=ok), 1), (dict(dg=ok), 1),
                         (dict(args=_norm(residual=None)), 1), (dict(lddx=60), 1), (dict(dn=ok, lddn=60), 1), (dict(dw=ok + 8), 1),
-                        (dict(s=None), 3), (dict(n=16), 3), (dict(s=ok + 8), 3)):
+                        (dict(s=None), 3), (dict(n=16), 3), (dict(s=ok + 8), 3), (dict(ws=None), 3), (dict(ws_bytes=255), 3)):
         assert lib.b200q_block_norm_backward(*{**good, **bad}.values()) == status, bad
     assert lib.b200q_block_norm_scratch_bytes(4, 60, 0) == 0 and lib.b200q_block_norm_scratch_bytes(4, 64, 3) == 0
     assert lib.b200q_block_norm_scratch_bytes(4, 64, 2) > 0

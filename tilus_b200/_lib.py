@@ -120,7 +120,7 @@ SYMBOLS = {
     "b200q_block_norm": (_i, [ctypes.POINTER(BlockNorm), _vp, _ll, _vp, _vp, _vp, _ll, _vp]),
     "b200q_block_norm_scratch_bytes": (_sz, [_i, _i, _i]),
     "b200q_block_norm_backward": (_i, [ctypes.POINTER(BlockNorm), _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp,
-                                       _sz, _vp]),
+                                       _sz, _vp, _sz, _vp]),
     "b200q_device_status": (_i, [_vp, ctypes.POINTER(ctypes.c_int32 * 4), _vp]),
 }
 

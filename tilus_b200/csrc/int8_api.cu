@@ -315,6 +315,7 @@ int b200q_block_norm(const b200q_block_norm_t* a, void* x, long long ldx, void* 
   p.tokens_per_gate = a->gates > 0 ? a->tokens / a->gates : a->tokens;
   p.ldb = a->ldb; p.ldr = a->ldr; p.ldg = a->ldg; p.ldx = ldx; p.ldn = ldn;
   p.scale = a->residual_scale; p.eps = a->eps;
+  p.sms = device_info().sm_count;
   const cudaError_t e = norm_launch(p, a->act_dtype, a->residual_f32 != 0, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? ST_OK : cuda_failed((int)e);
 }
@@ -329,7 +330,8 @@ size_t b200q_block_norm_scratch_bytes(int tokens, int hidden, int gates) {
 
 int b200q_block_norm_backward(const b200q_block_norm_t* a, const void* grad_x, long long lddx, const void* grad_new, long long lddn,
                               void* grad_block, long long lddb, void* grad_residual, long long lddr, float* grad_weight,
-                              float* grad_post, float* grad_gate, void* scratch, size_t scratch_bytes, void* stream) {
+                              float* grad_post, float* grad_gate, void* scratch, size_t scratch_bytes, void* workspace,
+                              size_t workspace_bytes, void* stream) {
   const int st = check_norm(a);
   if (st != ST_OK) return st;
   if (!grad_x || !grad_block || !grad_weight || (grad_post == nullptr) != (a->post_weight == nullptr) ||
@@ -342,7 +344,9 @@ int b200q_block_norm_backward(const b200q_block_norm_t* a, const void* grad_x, l
     return ST_INVALID_ARG;
   if (!scratch || misaligned(scratch, 16) || scratch_bytes < b200q_block_norm_scratch_bytes(a->tokens, a->hidden, a->gates))
     return ST_WORKSPACE;
+  if (!workspace || workspace_bytes < WS_HEADER_BYTES || misaligned(workspace, 256)) return ST_WORKSPACE;
   NormBackwardParams p = {};
+  p.status = static_cast<int*>(workspace);
   p.block = static_cast<const unsigned short*>(a->block);
   p.weight = static_cast<const unsigned short*>(a->weight);
   p.post = static_cast<const unsigned short*>(a->post_weight);

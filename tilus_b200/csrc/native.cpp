@@ -645,6 +645,9 @@ PyObject* block_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs
     const size_t need = g_norm_scratch((int)T, (int)D, n.c.gates);
     if (need == 0) return raise_status(B200Q_ERR_UNSUPPORTED);
     const at::Tensor scratch = at::detail::empty_cuda({(int64_t)need}, at::kByte, dev, std::nullopt);
+    const at::Tensor ws = workspace_of(dev.index(), stream, 256);
+    void* wsp = ws.mutable_data_ptr();
+    const size_t ws_bytes = (size_t)ws.numel();
     void *b = gb.mutable_data_ptr(), *r = n.residual ? gr.mutable_data_ptr() : nullptr, *s = scratch.mutable_data_ptr();
     float *w = gw.mutable_data_ptr<float>(), *p = n.post ? gp.mutable_data_ptr<float>() : nullptr;
     float* g = n.gate ? gg.mutable_data_ptr<float>() : nullptr;
@@ -653,7 +656,7 @@ PyObject* block_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs
     int st;
     {
       const NoGil unlocked;
-      st = g_norm_backward(&n.c, dxp, lddx, dnp, lddn, b, D, r, D, w, p, g, s, need, stream);
+      st = g_norm_backward(&n.c, dxp, lddx, dnp, lddn, b, D, r, D, w, p, g, s, need, wsp, ws_bytes, stream);
     }
     if (st != 0) return raise_status(st);
   } else {

@@ -4,7 +4,12 @@
 
 namespace b200q {
 
+constexpr int NORM_ROWS_FROM = 888;   // rows from which a block norm has its rows copied ahead (three to a CTA)
+constexpr int NORM_ROWS_STAGES = 4;   // rows in shared memory then
 constexpr int NORM_BACK_THREADS = 512;  // of an SM in the gradient's kernel, which takes up to 128 registers a thread
+
+constexpr int NORM_BACK_STAGES = 4;     // rows in shared memory
+constexpr int NORM_BACK_ROWS = 2;       // rows of a CTA at least, whose sums over them are as many bytes as six rows of a 16-bit type
 
 struct CastIntParams {
   const unsigned short* x;  // [T, D], row stride ldx, fp16 or bf16
@@ -27,6 +32,7 @@ struct NormParams {
   int T, D, tokens_per_gate;
   long long ldb, ldr, ldg, ldx, ldn;                   // row strides of block, residual, gate, x / x_int, new_residual
   float scale, eps;
+  int sms;                                             // of the GPU
 };
 struct NormBackwardParams {
   const unsigned short *block, *weight, *post, *gate, *grad_x;
@@ -35,6 +41,7 @@ struct NormBackwardParams {
   void* grad_residual;              // null: not wanted
   float *grad_weight, *grad_post, *grad_gate;  // [D], [D], [gates, D] fp32
   float* partial;                   // [CTAs][2 or 3][D]
+  int* status;                      // workspace status header
   int T, D, gates, tokens_per_gate;
   int ctas_per_gate, grid;          // CTAs that share a gate's rows; several gates to a CTA where it is 1
   int threads, vectors, stages, smem;  // threads of a row, its vectors of a thread, rows in shared memory and their bytes

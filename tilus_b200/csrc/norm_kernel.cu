@@ -124,6 +124,24 @@ __device__ __forceinline__ float row_sum(float x, float* slots, bool warp_row) {
   }
   return x;
 }
+// two sums over a CTA of up to 16 warps: a warp's shuffles after the first serve both
+__device__ __forceinline__ void row_sum2(float (&x)[2], float* slots) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float give = lane & 16 ? x[0] : x[1], mine = lane & 16 ? x[1] : x[0];
+  float y = mine + __shfl_xor_sync(0xffffffffu, give, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+  if ((lane & 15) == 0) slots[(lane & 16) + warp] = y;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    x[j] = 0.f;
+    for (int i = 0; i < (int)blockDim.x / 32; i += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(slots + 16 * j + i);
+      x[j] += (s.x + s.y) + (s.z + s.w);
+    }
+  }
+}
 __device__ __forceinline__ uint32_t row_max(uint32_t x, uint32_t* slots, bool warp_row) {
   x = __reduce_max_sync(0xffffffffu, x);
   if (warp_row) return x;
@@ -142,6 +160,21 @@ __device__ __forceinline__ void clear_slots(float (&slots)[N][32]) {
   if (threadIdx.x < 32 && threadIdx.x >= blockDim.x / 32)
 #pragma unroll
     for (int i = 0; i < N; ++i) slots[i][threadIdx.x] = 0.f;
+}
+
+// ---- rows copied ahead ----------------------------------------------------------------------------------
+// (16 bytes by the thread that will read them, so that nobody waits for anybody's copies)
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// a row or part of one, by the copy engine; the barrier counts its bytes
+__device__ __forceinline__ void copy_row(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes),
+               "r"(bar) : "memory");
+}
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() {  // all but the latest groups of this thread's have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
 // ---- per-token int8 cast --------------------------------------------------------------------------------
@@ -330,6 +363,148 @@ __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_kernel(const NormPar
   }
 }
 
+// The same for many rows of 2056 to 4096 channels with a 16-bit residual: each CTA takes every gridDim.x-th row, keeps the weights of its
+// threads' channels in registers and has the next rows copied to shared memory ahead of their turn; a row's reduction takes the next
+// row's sum of block block along.  4096 x 4096, us, a CTA to each row / this: with both norms 28.3 / 25.2, with one 24.4 / 22.7, of
+// a floor of 20.8.  (Wider rows and 32-bit residuals leave too few rows on an SM for that: 4097 x 8192 with a 32-bit one 69 / 84.)
+template <int ACT>
+__global__ void __launch_bounds__(256, 2) norm_rows_kernel(const NormParams p) {
+  extern __shared__ __align__(16) unsigned char rows_smem[];
+  __shared__ __align__(16) float slots[2][32], slots_block[32], slots_top[2][32];
+  constexpr int V = 2;
+  start_behind();
+  if (threadIdx.x < 32) {  // (words of warps that are not there stay zero)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) slots[i][threadIdx.x] = slots_top[i][threadIdx.x] = 0.f;
+    slots_block[threadIdx.x] = 0.f;
+  }
+  __syncthreads();
+  const int me = threadIdx.x, tpr = blockDim.x, nvec = p.D / 8;
+  const float inv_d = 1.0f / (float)p.D;
+  const F2 zero = both(0.f), scale = both(p.scale);
+  // [stage][block, residual][vector][thread], 16 bytes each
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rows_smem) + (uint32_t)me * 16u;
+  const uint32_t unit = (uint32_t)tpr * 16u, stage = unit * (2 * V), ring_end = ring + stage * NORM_ROWS_STAGES;
+  auto at = [&](uint32_t s, int u, int i) { return s + unit * (uint32_t)(u * V + i); };
+  auto load = [&](const unsigned short* from, int i) {
+    const int v = me + i * tpr;
+    return v < nvec ? *reinterpret_cast<const uint4*>(from + v * 8) : make_uint4(0, 0, 0, 0);
+  };
+  uint4 w_post[V], w_gate[V], w_norm[V];
+  const bool one_gate = p.tokens_per_gate >= p.T;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (p.post) w_post[i] = load(p.post, i);
+    if (p.gate && one_gate) w_gate[i] = load(p.gate, i);
+    w_norm[i] = load(p.weight, i);
+  }
+  int ask = blockIdx.x;
+  uint32_t ask_at = ring;
+  auto fetch = [&]() {
+    if (ask < p.T) {
+      const char* b = reinterpret_cast<const char*>(p.block + ask * p.ldb) + me * 16;
+      const char* r = static_cast<const char*>(p.residual) + (ask * p.ldr + me * 8) * 2;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (me + i * tpr < nvec) {
+          copy16(at(ask_at, 0, i), b + i * unit);
+          if (p.residual) copy16(at(ask_at, 1, i), r + i * unit);
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ask += gridDim.x;
+    ask_at = ask_at + stage == ring_end ? ring : ask_at + stage;
+  };
+  auto block_square = [&](uint32_t s) {
+    F2 x = zero;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (me + i * tpr < nvec) {
+        F2 b[4];
+        unpack8<ACT>(lds_u4(at(s, 0, i)), b);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x = fma2(b[k], b[k], x);
+      }
+    return sum(x);
+  };
+  for (int n = 0; n < NORM_ROWS_STAGES - 1; ++n) fetch();
+  float s1 = 1.f;
+  if (p.post) {
+    copies_wait<NORM_ROWS_STAGES - 2>();
+    s1 = rsqrtf(row_sum(block_square(ring), slots_block, false) * inv_d + p.eps);
+  }
+  uint32_t s = ring;
+  int turn = 0;
+  for (int t = blockIdx.x; t < p.T; t += gridDim.x, turn ^= 1) {
+    const uint32_t next = s + stage == ring_end ? ring : s + stage;
+    fetch();
+    copies_wait<NORM_ROWS_STAGES - 2>();
+    const unsigned short* gate = p.gate ? p.gate + (t / p.tokens_per_gate) * p.ldg : nullptr;
+    F2 r[V][4], rr = zero;
+    const F2 s1_2 = both(s1);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int v = me + i * tpr;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[i][k] = zero;
+      if (v < nvec) {
+        F2 q[4];
+        unpack8<ACT>(lds_u4(at(s, 0, i)), r[i]);
+        if (p.post) {
+          unpack8<ACT>(w_post[i], q);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) r[i][k] = r[i][k] * (s1_2 * q[k]);
+        }
+        if (gate) {
+          unpack8<ACT>(one_gate ? w_gate[i] : load(gate, i), q);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) r[i][k] = r[i][k] * q[k];
+        }
+        if (p.residual) {
+          unpack8<ACT>(lds_u4(at(s, 1, i)), q);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) r[i][k] = fma2(scale, q[k], r[i][k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rr = fma2(r[i][k], r[i][k], rr);
+        Wide<ACT, false>::store(p.new_residual, t * p.ldn + v * 8, r[i]);
+      }
+    }
+    float x[2] = {sum(rr), p.post && t + (int)gridDim.x < p.T ? block_square(next) : 0.f};
+    row_sum2(x, slots[turn]);
+    const F2 inv = both(rsqrtf(x[0] * inv_d + p.eps));
+    if (p.post) s1 = rsqrtf(x[1] * inv_d + p.eps);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int v = me + i * tpr;
+      F2 w[4];
+      unpack8<ACT>(w_norm[i], w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[i][k] = r[i][k] * (inv * w[k]);
+      const uint4 out = pack8<ACT>(r[i]);
+      if (p.x) {
+        if (v < nvec) *reinterpret_cast<uint4*>(p.x + t * p.ldx + v * 8) = out;
+      } else {
+        unpack8<ACT>(out, r[i]);
+        if (v < nvec) bits = top_bits<ACT>(bits, out);
+      }
+    }
+    if (!p.x) {
+      float sf, qinv;
+      int8_scale(__uint_as_float(row_max(top_value<ACT>(bits), reinterpret_cast<uint32_t*>(slots_top[turn]), false)), &sf, &qinv);
+      if (me == 0) p.x_sf[t] = sf;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int v = me + i * tpr;
+        if (v < nvec) *reinterpret_cast<uint2*>(p.x_int + t * p.ldx + v * 8) = int8_codes(r[i], qinv);
+      }
+    }
+    s = next;
+  }
+  copies_wait<0>();
+}
+
 // ---- its gradient ---------------------------------------------------------------------------------------
 // With s1, s2 the inverse deviations of the two norms, recomputed from the inputs (which have to be read anyway):
 //   bh = block s1, q = bh post gate (= gate n);  r = scale residual + q;  xh = r s2;  e = grad_x weight
@@ -341,17 +516,7 @@ __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_kernel(const NormPar
 //
 // A CTA takes a run of rows of one gate and keeps its share of the sums over rows in registers; a second kernel adds the CTAs' shares
 // in a fixed order, so that a call gives the same bits each time.  Rows are copied to shared memory ahead of their turn
-// (cp.async, each thread what it will read itself, so that nobody waits for anybody's copies): with a row at a time in registers and three
-// reductions 8192 x 5120 took 386 us, of a floor of 117.
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_wait(int pending) {  // all but the latest `pending` groups have landed
-  if (pending <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-  else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else asm volatile("cp.async.wait_group 2;" ::: "memory");
-}
-
+// by the copy engine: with a row at a time in registers and three reductions 8192 x 5120 took 386 us, of a floor of 117.
 // The sums of eight values over the CTA's threads, in every thread.  Halving exchanges: after the steps over 16, 8 and 4 lanes a lane
 // holds one value, lane >> 2; so a warp's part takes 9 shuffles instead of 40.  `slots`: 8 words a warp, of two sets in turn.
 __device__ __forceinline__ void sums8(float (&v)[8], float* slots) {
@@ -383,18 +548,27 @@ __device__ __forceinline__ void sums8(float (&v)[8], float* slots) {
 // V: vectors of eight channels to a thread.  Up to two, the weights of a thread's channels stay in registers too.
 template <int ACT, bool F32, int V>
 __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const NormBackwardParams p) {
-  extern __shared__ __align__(16) unsigned char rows_smem[];
+  extern __shared__ __align__(16) unsigned char rows_smem[];  // [stage]: a row of block, grad_x, residual, grad_new
   __shared__ __align__(16) float slots[2][8 * (NORM_BACK_THREADS / 32)], slots_block[1][32];
-  constexpr int WIDE = F32 ? 2 : 1, UNITS = 2 + 2 * WIDE;  // 16-byte units of a vector: block, grad_x, residual, grad_new
+  __shared__ uint64_t landed[NORM_BACK_STAGES];
+  __shared__ int gave_up;
+  constexpr int RB = F32 ? 4 : 2;
   constexpr bool KEEP = V <= 2;
   start_behind();
   clear_slots(slots_block);
   const int me = threadIdx.x, tpr = blockDim.x, nvec = p.D / 8;
   const float inv_d = 1.0f / (float)p.D;
   const F2 zero = both(0.f), scale = both(p.scale);
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rows_smem) + (uint32_t)me * 16u;
-  const uint32_t unit = (uint32_t)tpr * 16u, stage = unit * (UNITS * V), ring_end = ring + stage * (uint32_t)p.stages;
-  auto at = [&](uint32_t s, int u, int i) { return s + unit * (uint32_t)(u * V + i); };  // unit u of vector i in the stage at s
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rows_smem), landed_s = (uint32_t)__cvta_generic_to_shared(landed);
+  const uint32_t row16 = (uint32_t)p.D * 2u, row_wide = (uint32_t)p.D * RB, stage = 2u * row16 + 2u * row_wide;
+  if (me == 0) {
+    for (int i = 0; i < p.stages; ++i)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(landed_s + (uint32_t)i * 8u) : "memory");
+    gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
   auto load = [&](const unsigned short* from, int i, F2 (&w)[4]) {
     const int v = me + i * tpr;
     unpack8<ACT>(v < nvec ? *reinterpret_cast<const uint4*>(from + v * 8) : make_uint4(0, 0, 0, 0), w);
@@ -411,6 +585,26 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
       for (int k = 0; k < 4; ++k) pg[k] = pg[k] * x[k];
     }
   };
+  auto block_square = [&](uint32_t s) {
+    F2 x = zero;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (me + i * tpr < nvec) {
+        F2 b[4];
+        unpack8<ACT>(lds_u4(s + (uint32_t)(me + i * tpr) * 16u), b);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x = fma2(b[k], b[k], x);
+      }
+    return sum(x);
+  };
+  auto wide = [&](const void* there, uint32_t from, int v, F2 (&f)[4]) {
+    Wide<ACT, F32> w;
+    w.zero();
+    if (there)
+#pragma unroll
+      for (int h = 0; h < Wide<ACT, F32>::UNITS; ++h) w.v[h] = lds_u4(from + (uint32_t)v * (8u * RB) + (uint32_t)h * 16u);
+    w.get(f);
+  };
   F2 kept_w[KEEP ? V : 1][4], kept_pg[KEEP ? V : 1][4], gw[V][4], S[V][4];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -421,7 +615,8 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
   // Three stages and more: a row's reduction takes the next row's sum of block block along, whose copies have landed by then.
   const bool ahead = p.stages >= 3;
   const int part = (int)(blockIdx.x % p.ctas_per_gate), stride = (int)(gridDim.x / p.ctas_per_gate);
-  bool first_gate = true;
+  bool first_gate = true, good = true;
+  int lap = 0, at = 0;  // of the next row to be read: how often its stage has been used, and which
   for (int g = blockIdx.x / p.ctas_per_gate; g < p.gates; g += stride, first_gate = false) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -431,78 +626,53 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
     }
     const int r0 = (int)((long long)p.tokens_per_gate * part / p.ctas_per_gate);
     const int rows = (int)((long long)p.tokens_per_gate * (part + 1) / p.ctas_per_gate) - r0;
-    // this thread's first vector of the next row to be copied and of the next to be written
     const long long t0 = (long long)g * p.tokens_per_gate + r0;
-    const char* from_b = reinterpret_cast<const char*>(p.block + t0 * p.ldb) + me * 16;
-    const char* from_x = reinterpret_cast<const char*>(p.grad_x + t0 * p.lddx) + me * 16;
-    const char* from_r = static_cast<const char*>(p.residual) + (t0 * p.ldr + me * 8) * (F32 ? 4 : 2);
-    const char* from_n = static_cast<const char*>(p.grad_new) + (t0 * p.lddn + me * 8) * (F32 ? 4 : 2);
     long long to_b = t0 * p.lddb + me * 8, to_r = t0 * p.lddr + me * 8;
-    int asked = 0;
-    uint32_t ask_at = ring;
-    auto fetch = [&]() {  // the next row of this run, to the next stage
-      if (asked < rows) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (me + i * tpr < nvec) {
-            copy16(at(ask_at, 0, i), from_b + i * unit);
-            copy16(at(ask_at, 1, i), from_x + i * unit);
-#pragma unroll
-            for (int h = 0; h < WIDE; ++h) {
-              if (p.residual) copy16(at(ask_at, 2 + h, i), from_r + i * unit * WIDE + h * 16);
-              if (p.grad_new) copy16(at(ask_at, 2 + WIDE + h, i), from_n + i * unit * WIDE + h * 16);
-            }
-          }
-        }
-        from_b += p.ldb * 2; from_x += p.lddx * 2;
-        from_r += p.ldr * (F32 ? 4 : 2); from_n += p.lddn * (F32 ? 4 : 2);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+    // Thread 0 asks for rows, in order, the stages in turn from this run's first.
+    int asked = 0, ask_stage = at;
+    auto fetch = [&]() {
+      if (asked >= rows) return;
+      const long long t = t0 + asked;
+      const uint32_t bar = landed_s + (uint32_t)ask_stage * 8u, to = ring + (uint32_t)ask_stage * stage;
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                   "r"(2u * row16 + (p.residual ? row_wide : 0u) + (p.grad_new ? row_wide : 0u)) : "memory");
+      copy_row(to, p.block + t * p.ldb, row16, bar);
+      copy_row(to + row16, p.grad_x + t * p.lddx, row16, bar);
+      if (p.residual) copy_row(to + 2u * row16, static_cast<const char*>(p.residual) + t * p.ldr * RB, row_wide, bar);
+      if (p.grad_new) copy_row(to + 2u * row16 + row_wide, static_cast<const char*>(p.grad_new) + t * p.lddn * RB, row_wide, bar);
       ++asked;
-      ask_at = ask_at + stage == ring_end ? ring : ask_at + stage;
+      if (++ask_stage == p.stages) ask_stage = 0;
     };
-    auto block_square = [&](uint32_t s) {
-      F2 x = zero;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (me + i * tpr < nvec) {
-          F2 b[4];
-          unpack8<ACT>(lds_u4(at(s, 0, i)), b);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x = fma2(b[k], b[k], x);
-        }
-      return sum(x);
+    // A thread that has given up waits no more, but keeps in step with the others.
+    auto await = [&](int stage_i, int lap_i) {
+      if (good && !mbar_wait_bounded(landed_s + (uint32_t)stage_i * 8u, (uint32_t)lap_i & 1u)) {
+        good = false;
+        gave_up = 1;
+      }
     };
-    auto wide = [&](const void* there, uint32_t s, int u, int i, F2 (&f)[4]) {
-      Wide<ACT, F32> w;
-      w.zero();
-      if (there)
-#pragma unroll
-        for (int h = 0; h < WIDE; ++h) w.v[h] = lds_u4(at(s, u + h, i));
-      w.get(f);
-    };
-    for (int n = 0; n < p.stages - 1; ++n) fetch();
+    if (me == 0)
+      for (int n = 0; n < p.stages; ++n) fetch();
     float s1 = 1.f;
     if (ahead && p.post && rows > 0) {
-      copies_wait(p.stages - 2);
-      s1 = rsqrtf(row_sum(block_square(ring), slots_block[0], false) * inv_d + p.eps);
+      await(at, lap);
+      s1 = rsqrtf(row_sum(block_square(ring + (uint32_t)at * stage), slots_block[0], false) * inv_d + p.eps);
     }
-    uint32_t s = ring;
     for (int n = 0; n < rows; ++n) {
-      const uint32_t next = s + stage == ring_end ? ring : s + stage;
-      fetch();
-      copies_wait(ahead ? p.stages - 2 : p.stages - 1);
+      const uint32_t s = ring + (uint32_t)at * stage;
+      const int next = at + 1 == p.stages ? 0 : at + 1, next_lap = at + 1 == p.stages ? lap + 1 : lap;
+      if (!(ahead && p.post)) await(at, lap);  // (else the last row's turn has waited for it)
       if (!ahead && p.post) s1 = rsqrtf(row_sum(block_square(s), slots_block[0], false) * inv_d + p.eps);
       F2 rr = zero, er = zero, qn = zero, qe = zero, qr = zero;
       const F2 s1_2 = both(s1);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        if (me + i * tpr < nvec) {
+        const int v = me + i * tpr;
+        if (v < nvec) {
           F2 b[4], d[4], res[4], dn[4], w[4], pg[4];
-          unpack8<ACT>(lds_u4(at(s, 0, i)), b);
-          unpack8<ACT>(lds_u4(at(s, 1, i)), d);
-          wide(p.residual, s, 2, i, res);
-          wide(p.grad_new, s, 2 + WIDE, i, dn);
+          unpack8<ACT>(lds_u4(s + (uint32_t)v * 16u), b);
+          unpack8<ACT>(lds_u4(s + row16 + (uint32_t)v * 16u), d);
+          wide(p.residual, s + 2u * row16, v, res);
+          wide(p.grad_new, s + 2u * row16 + row_wide, v, dn);
           if constexpr (!KEEP) { load(p.weight, i, w); load_pg(g, i, pg); }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -517,8 +687,12 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
         }
       }
       float x[8] = {sum(rr), sum(er), sum(qn), sum(qe), sum(qr), 0.f, 0.f, 0.f};
-      if (ahead && p.post && n + 1 < rows) x[5] = block_square(next);
+      if (ahead && p.post && n + 1 < rows) {
+        await(next, next_lap);
+        x[5] = block_square(ring + (uint32_t)next * stage);
+      }
       sums8(x, slots[n & 1]);
+      if (me == 0 && n > 0 && p.stages > 1) fetch();  // every thread is done with the row before this one
       const float s2 = rsqrtf(x[0] * inv_d + p.eps), mean = x[1] * s2 * inv_d;                       // of e xh
       const float mean_q = p.post ? (x[2] + s2 * (x[3] - s2 * mean * x[4])) * inv_d : 0.f;           // of dr q
       const F2 s2_2 = both(s2), mean_2 = both(-mean), mean_q2 = both(-mean_q);
@@ -527,10 +701,10 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
         const int v = me + i * tpr;
         if (v < nvec) {
           F2 b[4], d[4], res[4], dn[4], w[4], pg[4], out[4];
-          unpack8<ACT>(lds_u4(at(s, 0, i)), b);
-          unpack8<ACT>(lds_u4(at(s, 1, i)), d);
-          wide(p.residual, s, 2, i, res);
-          wide(p.grad_new, s, 2 + WIDE, i, dn);
+          unpack8<ACT>(lds_u4(s + (uint32_t)v * 16u), b);
+          unpack8<ACT>(lds_u4(s + row16 + (uint32_t)v * 16u), d);
+          wide(p.residual, s + 2u * row16, v, res);
+          wide(p.grad_new, s + 2u * row16 + row_wide, v, dn);
           if constexpr (!KEEP) { load(p.weight, i, w); load_pg(g, i, pg); }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -548,7 +722,12 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
       }
       to_b += p.lddb; to_r += p.lddr;
       if (ahead && p.post) s1 = rsqrtf(x[5] * inv_d + p.eps);
-      s = next;
+      at = next;
+      lap = next_lap;
+      if (p.stages == 1) {  // the next row goes where this one was
+        __syncthreads();
+        if (me == 0) fetch();
+      }
     }
     // the gate's sums: its own gradient, and what its rows give post
 #pragma unroll
@@ -580,8 +759,21 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
         Wide<ACT, true>::store(p.partial, to, x);
       }
     }
-    copies_wait(0);   // (what was asked for past the run's end is nothing)
-    __syncthreads();  // the slots of this run's last row have been read
+    __syncthreads();  // the stages and slots of this run's last row have been read
+  }
+  if (gave_up) {
+    // The copies in flight get their chance to land before the CTA ends, and the sums are no numbers.
+    if (me == 0) {
+      for (int i = 0; i < p.stages; ++i) {
+        const int last = i < at ? lap : lap - 1;
+        if (last >= 0) mbar_wait_bounded(landed_s + (uint32_t)i * 8u, (uint32_t)last & 1u);
+      }
+      atomicExch(p.status, ST_DEVICE_TIMEOUT);
+      p.status[1] = 14;  // where: gradient of the block norm
+      p.status[2] = blockIdx.x;
+      p.status[3] = 0;
+    }
+    gw[0][0] = both(__int_as_float(0x7fc00000));
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -590,8 +782,8 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
   }
 }
 
-// The sums of the CTAs' shares: 32 columns a CTA, eight runs of CTAs' shares side by side, joined in order.  blockIdx.y: grad_weight,
-// grad_post, then one for each gate.
+// The sums of the CTAs' shares: 32 columns a CTA, eight runs of shares side by side, joined in order.  (With 32 runs to a CTA of 1024
+// threads 4096 x 4096 took 52.2 us, not 50.8.)  blockIdx.y: grad_weight, grad_post, then one for each gate.
 __global__ void __launch_bounds__(256) norm_sums_kernel(const NormBackwardParams p) {
   __shared__ float part[8][33];
   start_behind();
@@ -612,7 +804,7 @@ __global__ void __launch_bounds__(256) norm_sums_kernel(const NormBackwardParams
   float s = 0.f;
   if (col < p.D) {
     const int i0 = n * run / 8, i1 = n * (run + 1) / 8;
-#pragma unroll 8
+#pragma unroll 10
     for (int i = i0; i < i1; ++i) s += from[(long long)i * p.D + col];
   }
   part[run][threadIdx.x & 31] = s;
@@ -640,22 +832,23 @@ static cudaError_t launch_behind(Kernel kern, dim3 grid, int threads, int smem, 
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// Threads of a row and vectors of a thread: a warp for up to 512 channels, else a CTA.  Where rows are many, 256 threads with up to
+// Threads of a row and vectors of a thread: a warp for up to 512 channels (2048 where rows are many), else a CTA.  Where rows are many, 256 threads with up to
 // eight vectors, so that the steps of a reduction are shared by many channels; where they are few, as many as the row has.
 struct RowShape { int warp_rows, threads, vectors, ctas; };
-static RowShape row_shape(int T, int D, int most_vectors) {
+static RowShape row_shape(int T, int D, bool wide = false) {
   const int nvec = D / 8;
   RowShape s;
-  s.warp_rows = nvec <= 64 ? 1 : 0;
+  s.warp_rows = nvec <= (T > 1024 ? 256 : 64) ? 1 : 0;
   if (s.warp_rows) {
-    s.vectors = nvec <= 32 ? 1 : 2;
+    s.vectors = nvec <= 32 ? 1 : nvec <= 64 ? 2 : nvec <= 128 ? 4 : 8;
     s.threads = 128;
     s.ctas = (T + 3) / 4;
     return s;
   }
-  const int threads = T <= 296 ? 512 : 256;
+  // (4097 x 8192 with a 32-bit residual, us, with 256 threads / 512: 69.0 / 64.5; 4096 x 5120: 45.9 / 49.8; 2048 x 16384: 110 / 115)
+  const int threads = T <= 296 || (wide && nvec > 768 && nvec <= 1024) ? 512 : 256;
   s.vectors = 1;
-  while (s.vectors < most_vectors && s.vectors * threads < nvec) s.vectors *= 2;
+  while (s.vectors < 8 && s.vectors * threads < nvec) s.vectors *= 2;
   const int per = (nvec + s.vectors - 1) / s.vectors;
   s.threads = (per + 31) / 32 * 32;
   if (s.threads > 512) s.threads = 512;
@@ -665,7 +858,7 @@ static RowShape row_shape(int T, int D, int most_vectors) {
 
 template <int ACT>
 static cudaError_t cast_int_act(const CastIntParams& p, cudaStream_t stream) {
-  const RowShape s = row_shape(p.T, p.D, 8);
+  const RowShape s = row_shape(p.T, p.D);
   const dim3 grid((unsigned)s.ctas, 1, 1);
   switch (s.vectors) {
     case 1: return launch_behind(cast_int_kernel<ACT, 1>, grid, s.threads, 0, stream, p, s.warp_rows);
@@ -678,9 +871,21 @@ cudaError_t cast_int_launch(const CastIntParams& p, int act, cudaStream_t stream
   return act == 0 ? cast_int_act<0>(p, stream) : cast_int_act<1>(p, stream);
 }
 
+template <int ACT>
+static cudaError_t norm_rows(NormParams p, int threads, cudaStream_t stream) {
+  static std::atomic<bool> allowed[16];
+  const cudaError_t e = allow_smem(norm_rows_kernel<ACT>, allowed);
+  if (e != cudaSuccess) return e;
+  const int most = 2 * p.sms;  // two CTAs to an SM, by registers and shared memory
+  return launch_behind(norm_rows_kernel<ACT>, dim3((unsigned)(p.T < most ? p.T : most), 1, 1), threads,
+                       NORM_ROWS_STAGES * 2 * 2 * threads * 16, stream, p);
+}
 template <int ACT, bool F32>
 static cudaError_t norm_type(const NormParams& p, cudaStream_t stream) {
-  const RowShape s = row_shape(p.T, p.D, 8);
+  const int nvec = p.D / 8;
+  if constexpr (!F32)
+    if (nvec > 256 && nvec <= 512 && p.T >= NORM_ROWS_FROM) return norm_rows<ACT>(p, (nvec + 63) / 64 * 32, stream);
+  const RowShape s = row_shape(p.T, p.D, F32);
   const dim3 grid((unsigned)s.ctas, 1, 1);
   switch (s.vectors) {
     case 1: return launch_behind(norm_kernel<ACT, F32, 1>, grid, s.threads, 0, stream, p, s.warp_rows);
@@ -716,18 +921,20 @@ static cudaError_t backward_type(const NormBackwardParams& p, cudaStream_t strea
 // The shape of the gradient's launch: threads and vectors of a row, CTAs (512 threads to an SM), and stages for the rows ahead.
 void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gate, int sms, int max_smem, NormBackwardParams* p) {
   const int nvec = D / 8;
-  p->vectors = nvec <= 256 ? 1 : nvec <= 1024 ? 2 : 4;
+  const bool few = (long long)gates * tokens_per_gate <= 16ll * sms;
+  p->vectors = nvec <= (few ? 512 : 256) ? 1 : nvec <= 1024 ? 2 : 4;
   p->threads = ((nvec + p->vectors - 1) / p->vectors + 31) / 32 * 32;
-  const int per_sm = NORM_BACK_THREADS / p->threads < 4 ? NORM_BACK_THREADS / p->threads : 4, most = sms * per_sm;
+  const int per_sm = NORM_BACK_THREADS / p->threads < 8 ? NORM_BACK_THREADS / p->threads : 8, most = sms * per_sm;
+  const int runs = (tokens_per_gate + NORM_BACK_ROWS - 1) / NORM_BACK_ROWS;  // that a gate's rows are enough for
   if (gates >= most) {
     p->ctas_per_gate = 1;
     p->grid = most;
   } else {
-    p->ctas_per_gate = most / gates < tokens_per_gate ? most / gates : tokens_per_gate;
+    p->ctas_per_gate = most / gates < runs ? most / gates : runs;
     p->grid = gates * p->ctas_per_gate;
   }
-  const int stage = p->vectors * p->threads * 16 * (residual_f32 ? 6 : 4), room = (max_smem + 1024) / per_sm - 1024 - 2048;
-  p->stages = room / stage > 4 ? 4 : room / stage;
+  const int stage = D * (residual_f32 ? 12 : 8), room = (max_smem + 1024) / per_sm - 1024 - 2048;
+  p->stages = room / stage > NORM_BACK_STAGES ? NORM_BACK_STAGES : room / stage;
   p->smem = p->stages * stage;
 }
 cudaError_t norm_backward_launch(const NormBackwardParams& p, int act, bool residual_f32, cudaStream_t stream) {
