@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(1024) cast_int_kernel(const CastIntParams p, c
 
 // ---- block norm -------------------------------------------------------------------------------------------
 template <int ACT, bool F32, int V>
-__global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_kernel(const NormParams p, const int warp_rows) {
+__global__ void __launch_bounds__(V <= 2 ? 1024 : 512, V == 4 && !F32 ? 2 : 1) norm_kernel(const NormParams p, const int warp_rows) {
   __shared__ __align__(16) float slots[3][32];
   start_behind();
   const bool warp_row = warp_rows != 0;
@@ -835,7 +835,7 @@ static cudaError_t launch_behind(Kernel kern, dim3 grid, int threads, int smem, 
 // Threads of a row and vectors of a thread: a warp for up to 512 channels (2048 where rows are many), else a CTA.  Where rows are many, 256 threads with up to
 // eight vectors, so that the steps of a reduction are shared by many channels; where they are few, as many as the row has.
 struct RowShape { int warp_rows, threads, vectors, ctas; };
-static RowShape row_shape(int T, int D, bool wide = false) {
+static RowShape row_shape(int T, int D) {
   const int nvec = D / 8;
   RowShape s;
   s.warp_rows = nvec <= (T > 1024 ? 256 : 64) ? 1 : 0;
@@ -845,8 +845,9 @@ static RowShape row_shape(int T, int D, bool wide = false) {
     s.ctas = (T + 3) / 4;
     return s;
   }
-  // (4097 x 8192 with a 32-bit residual, us, with 256 threads / 512: 69.0 / 64.5; 4096 x 5120: 45.9 / 49.8; 2048 x 16384: 110 / 115)
-  const int threads = T <= 296 || (wide && nvec > 768 && nvec <= 1024) ? 512 : 256;
+  // (us, 256 threads / 512: 4096 x 8192 53.2 / 48.3, with a 32-bit residual 69.0 / 61.7; 4096 x 6144 44.6 / 48.3, 55.0 / 61.5; 2048 x 16384
+  // 54.4 / 69.8)
+  const int threads = T <= 296 || (nvec > 768 && nvec <= 1024) ? 512 : 256;
   s.vectors = 1;
   while (s.vectors < 8 && s.vectors * threads < nvec) s.vectors *= 2;
   const int per = (nvec + s.vectors - 1) / s.vectors;
@@ -885,7 +886,7 @@ static cudaError_t norm_type(const NormParams& p, cudaStream_t stream) {
   const int nvec = p.D / 8;
   if constexpr (!F32)
     if (nvec > 256 && nvec <= 512 && p.T >= NORM_ROWS_FROM) return norm_rows<ACT>(p, (nvec + 63) / 64 * 32, stream);
-  const RowShape s = row_shape(p.T, p.D, F32);
+  const RowShape s = row_shape(p.T, p.D);
   const dim3 grid((unsigned)s.ctas, 1, 1);
   switch (s.vectors) {
     case 1: return launch_behind(norm_kernel<ACT, F32, 1>, grid, s.threads, 0, stream, p, s.warp_rows);
