@@ -132,7 +132,7 @@ def test_every_plan_gives_the_same_bits(M, N, K, gated):
     edits += [dict(kernel=1, width=w, ctas=4, tail_rows=t) for w in (256, 128) for t in (1, 5, 16) if t < M]
     if M <= 256:
         edits += [dict(kernel=2, tail_rows=0, width=w * c, cluster=c, stages=s)
-                  for w, c, s in ((16, 1, 1), (48, 1, 3), (80, 1, 3), (128, 1, 2), (16, 2, 4), (64, 2, 1), (16, 3, 2), (32, 4, 3),
+                  for w, c, s in ((16, 1, 1), (48, 1, 3), (24, 1, 2), (56, 1, 2), (120, 1, 2), (80, 1, 3), (128, 1, 2), (16, 2, 4), (64, 2, 1), (16, 3, 2), (32, 4, 3),
                                   (16, 5, 5), (16, 7, 2), (16, 8, 4), (16, 1, 16))
                   if c <= -(-K // 128) and (M <= 64 or c < 5 and s < 16)]  # (what shared memory holds)
     if M <= 16:
@@ -154,7 +154,7 @@ def test_plans_that_cannot_run_are_refused():
         assert _planned(a, b, a_sf, b_sf, out, False, **edit) == _lib.ST_OK
     for kernel, edit in ((1, dict(kernel=0)), (1, dict(kernel=4)), (1, dict(width=64)), (1, dict(ctas=3)), (1, dict(ctas=0)),
                          (1, dict(ctas=4096)), (1, dict(tail_rows=8)), (1, dict(tail_rows=-1)), (2, dict(cluster=9)),
-                         (2, dict(cluster=5)), (2, dict(cluster=0)), (2, dict(stages=0)), (2, dict(stages=17)), (2, dict(width=72)),
+                         (2, dict(cluster=5)), (2, dict(cluster=0)), (2, dict(stages=0)), (2, dict(stages=17)), (2, dict(width=72)), (2, dict(cluster=1, width=60)),
                          (2, dict(width=48)), (2, dict(width=512)), (2, dict(tail_rows=1)), (3, dict(ctas=0)), (3, dict(tail_rows=1))):
         assert _planned(a, b, a_sf, b_sf, out, False, **{**good[kernel], **edit}) == _lib.ST_UNSUPPORTED, edit
     a, b, a_sf, b_sf = _operands(17, 256, 512)

@@ -27,12 +27,13 @@ static int pair_tiles(int M, int N, bool gated, int cols) {
   return (int)(((long long)M + 255) / 256 * ((N + per - 1) / per));
 }
 // Output columns of a stream kernel's tile with `s` CTAs to a cluster: an equal share of N for all SMs in as few rounds as the
-// tensor core's 256 columns allow, in units of 16 for each CTA.
+// tensor core's 256 columns allow, in units of 8, or of 16 for each CTA of a cluster.
+static int stream_unit(int s) { return s == 1 ? 8 : 16 * s; }
 static int stream_width(int N, bool gated, int s, int sms) {
-  const int most = (gated ? 128 : 256) / (16 * s) * (16 * s), groups = sms / s;
+  const int unit = stream_unit(s), most = (gated ? 128 : 256) / unit * unit, groups = sms / s;
   const int rounds = (N + most * groups - 1) / (most * groups);
-  const int share = (N + rounds * groups - 1) / (rounds * groups);
-  return (share + 16 * s - 1) / (16 * s) * (16 * s);
+  const int share = (N + rounds * groups - 1) / (rounds * groups), width = (share + unit - 1) / unit * unit;
+  return width < 16 ? 16 : width;
 }
 static int stream_stages(int M, int b_rows, int s, int budget) {
   int stages = 16;
@@ -45,30 +46,39 @@ static int stream_stages(int M, int b_rows, int s, int budget) {
 constexpr double kHbm = 6465.5e3;  // bytes a us
 
 // Reading B at five sixths of the memory's rate up to eight rows of A (with twice as many, whose loads are as many as B's, at three
-// fifths), but no less than the latency of each round of a CTA.
-static double row_cost(int M, double b_bytes, int rounds) {
-  const double memory = 1.6 + b_bytes / kHbm * (M <= 8 ? 1.2 : 1.62), latency = 0.4 + rounds * (M <= 8 ? 1.5 : 2.0);
+// fifths), but no less than the latency of each round of a CTA and of each 4096 bytes of K in it.
+static double row_cost(int M, double b_bytes, int rounds, int K) {
+  const bool few = M <= 8;
+  const int more = (K - 1) / 4096;
+  const double memory = 1.6 + b_bytes / kHbm * (few ? 1.2 : 1.62);
+  const double latency = 0.4 + rounds * (few ? 1.5 + 1.7 * more : 2.0 + 2.8 * more);
   return memory > latency ? memory : latency;
 }
 
 // A piece of 128 bytes of K takes what the slowest of three takes: reading B, bringing both operands' rows to the SM (121 GB/s a SM),
 // and the tensor core's reading them (about as fast, but whole accumulators' rows of A).  A cluster's exchange goes by its size
-// and rows: 64 x 4096 x 14336 takes 20.1 us alone, 14.5 in pairs, 15.3 in fours; 128 rows 20.7, 17.1, 19.4.
-static double stream_cost(int M, int b_rows, int ctas, int s, int kblocks, const DeviceInfo& di) {
-  const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, rounds = (ctas + di.sm_count - 1) / di.sm_count;
-  const int busy = ctas < di.sm_count ? ctas : di.sm_count;
-  const double tensor = accs * (128 + b_rows) * 1.05e-3, in = (rows + b_rows) * 1.05e-3, memory = 128.0 * b_rows * busy / kHbm * 1.08;
+// and rows: 64 x 4096 x 14336 takes 20.1 us alone, 14.5 in pairs, 15.3 in fours; 128 rows 20.7, 17.1, 19.4.  Two CTAs to an SM
+// (`per` 2) share it, but one starts and ends under the other: 8 x 28672 gated 22.5 us with one, 20.6 with two.
+static double stream_cost(int M, int b_rows, int ctas, int s, int per, int kblocks, const DeviceInfo& di) {
+  const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, slots = per * di.sm_count, rounds = (ctas + slots - 1) / slots;
+  const int busy = ctas < slots ? ctas : slots;
+  const double tensor = per * accs * (128 + b_rows) * 1.05e-3, in = per * (rows + b_rows) * 1.05e-3;
+  const double memory = 128.0 * b_rows * busy / kHbm * (per == 1 ? 1.08 : 1.03);
   const double piece = tensor > in ? (tensor > memory ? tensor : memory) : (in > memory ? in : memory);
-  return 2.8 + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.25 * s + 0.012 * s * M : 0.0) + 0.004 * M;
+  return (per == 1 ? 2.8 : 2.6) + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.25 * s + 0.012 * s * M : 0.0) +
+         0.004 * per * M;
 }
 
 // A piece of a tile of 256 x 256 takes 0.30 us (0.28 at rest, 0.35 under the power limit), of 256 x 128 two thirds: its operands come
 // through the same SM.  A tile takes no less than its outputs do, 3.1 and 1.9 us (gated 2.6: half
-// of the writers have none of a narrow tile).  Up front, and for the last tile's outputs: 5.6 and 3.9.
-static double pair_cost(int tiles, bool gated, int cols, int kblocks, const DeviceInfo& di) {
+// of the writers have none of a narrow tile).  Up front, and for the last tile's outputs: 5.6 and 3.9.  And
+// B has to be read.
+static double pair_cost(int tiles, bool gated, int cols, int kblocks, double b_bytes, const DeviceInfo& di) {
   const int pairs = di.sm_count / 2, rounds = (tiles + pairs - 1) / pairs;
   const double products = kblocks * (cols == 256 ? 0.30 : 0.195), outputs = cols == 256 ? 3.1 : gated ? 2.6 : 1.9;
-  return (cols == 256 ? 5.6 : 3.9) + products + (rounds - 1) * (products > outputs ? products : outputs);
+  const double start = cols == 256 ? 5.6 : 3.9, all = products + (rounds - 1) * (products > outputs ? products : outputs);
+  const double memory = 1.15 * b_bytes / kHbm;
+  return start + (all > memory ? all : memory);
 }
 
 static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) {
@@ -81,29 +91,31 @@ static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) 
   for (int cols = 256; cols >= 128; cols -= 128)
     for (int tail = 0; tail <= past; tail += past > 0 ? past : 1) {
       const int tiles = pair_tiles(M - tail, N, gated, cols), items = N / (gated ? 8 : 16), sms = di.sm_count;
-      double cost = pair_cost(tiles, gated, cols, kblocks, di);
-      if (tail > 0) cost += 0.7 * row_cost(tail, (double)(gated ? 2 : 1) * N * K, (items + 2 * sms - 1) / (2 * sms));
+      double cost = pair_cost(tiles, gated, cols, kblocks, (double)(gated ? 2 : 1) * N * K, di);
+      if (tail > 0) cost += 0.7 * row_cost(tail, (double)(gated ? 2 : 1) * N * K, (items + 2 * sms - 1) / (2 * sms), K);
       if (cost >= best) continue;
       best = cost;
       *pl = {1, 256, cols, 2, cols == 256 ? 6 : 8, 2 * (tiles < sms / 2 ? tiles : sms / 2), tail};
     }
   if (M > kStreamRows) return;
-  for (int s = 1; s <= 8 && 4 * (s - 1) <= kblocks; s *= 2) {
-    const int width = stream_width(N, gated, s, di.sm_count), b_rows = gated ? 2 * width : width;
-    const int ctas = (N + width - 1) / width * s;
-    const double cost = stream_cost(M, b_rows, ctas, s, kblocks, di);
-    if (cost >= best) continue;
-    // half an SM's shared memory where that is depth enough for the length of K: a CTA of the stream's next launch has room next to it
-    // then (126 x 9376 x 704, us with 4 stages / 9 of a whole SM's: 4.6 / 5.4; 100 x 11008 x 4224 with 4 / 8: 14.0 / 11.5)
-    int stages = stream_stages(M, b_rows, s, 113 * 1024);
-    if (stages < (kblocks <= 8 * s ? 3 : 8)) stages = stream_stages(M, b_rows, s, di.max_smem);
-    if (stages < 2) continue;
-    best = cost;
-    *pl = {2, (M + 15) / 16 * 16, width, s, stages, ctas, 0};
-  }
+  for (int s = 1; s <= 8 && 4 * (s - 1) <= kblocks; s *= 2)
+    for (int per = s == 1 && kblocks >= 16 ? 2 : 1; per >= 1; --per) {
+      const int width = stream_width(N, gated, s, per * di.sm_count), b_rows = gated ? 2 * width : width;
+      const int ctas = (N + width - 1) / width * s;
+      const double cost = stream_cost(M, b_rows, ctas, s, per, kblocks, di);
+      if (cost >= best) continue;
+      // half an SM's shared memory for one of two CTAs, or where that is depth enough for the length of K: a CTA of the stream's next
+      // launch has room next to it then (126 x 9376 x 704, us with 4 stages / 9 of a whole SM's: 4.6 / 5.4; 100 x 11008 x 4224 with 4 / 8:
+      // 14.0 / 11.5)
+      int stages = stream_stages(M, b_rows, s, 113 * 1024);
+      if (per == 1 && stages < (kblocks <= 8 * s ? 3 : 8)) stages = stream_stages(M, b_rows, s, di.max_smem);
+      if (stages < (per == 1 ? 2 : 4)) continue;
+      best = cost;
+      *pl = {2, (M + 15) / 16 * 16, width, s, stages, ctas, 0};
+    }
   if (M <= 16) {
     const int items = N / (gated ? 8 : 16);
-    const double cost = row_cost(M, (double)(gated ? 2 : 1) * N * K, (items + 2 * di.sm_count - 1) / (2 * di.sm_count));
+    const double cost = row_cost(M, (double)(gated ? 2 : 1) * N * K, (items + 2 * di.sm_count - 1) / (2 * di.sm_count), K);
     if (cost < best) *pl = {3, M, gated ? 8 : 16, 1, 1, items < 2 * di.sm_count ? items : 2 * di.sm_count, 0};
   }
 }
@@ -206,7 +218,7 @@ static bool igemm_plan_ok(int M, int N, int K, bool gated, b200q_igemm_plan_t* p
   if (pl->kernel != 2 || M > kStreamRows) return false;
   pl->rows = (M + 15) / 16 * 16;
   if (pl->cluster < 1 || pl->cluster > 8 || pl->cluster > igemm_kblocks(K)) return false;
-  if (pl->width < 16 || pl->width > (gated ? 128 : 256) || pl->width % (16 * pl->cluster) != 0) return false;
+  if (pl->width < 16 || pl->width > (gated ? 128 : 256) || pl->width % stream_unit(pl->cluster) != 0) return false;
   pl->ctas = (N + pl->width - 1) / pl->width * pl->cluster;
   return pl->stages >= 1 && pl->stages <= 16 &&
          int8_stream_smem_bytes(M, gated ? 2 * pl->width : pl->width, pl->cluster, pl->stages) <= di.max_smem;

@@ -407,10 +407,11 @@ __global__ void __launch_bounds__(S_THREADS)
   const int n0 = (S > 1 ? blockIdx.x / S : blockIdx.x) * p.width;
   const int kb0 = (int)((long long)p.kblocks * rank / S), kb1 = (int)((long long)p.kblocks * (rank + 1) / S);
   const int b_rows = GATED ? 2 * p.width : p.width;
+  const int mma_n = (b_rows + 15) / 16 * 16;  // (what is past B's rows of a stage is rows of A: columns that nobody reads)
   const uint32_t b_bytes = (uint32_t)b_rows * 128u, stage_bytes = b_bytes + (uint32_t)p.rows * 128u;
   const int accs = p.rows > 128 ? 2 : 1;
   uint32_t cols = 32;  // of tensor memory: a power of two
-  while (cols < (uint32_t)(accs * b_rows)) cols *= 2;
+  while (cols < (uint32_t)(accs * mma_n)) cols *= 2;
   const int pitch = stream_inbox_pitch(b_rows, S);
   const bool apart = stream_inbox_bytes(p.M, b_rows, S) <= S_INBOX_APART;
   const uint32_t inbox = apart ? ring + (uint32_t)stream_ring_bytes(p.rows, b_rows, p.stages) : ring;
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(S_THREADS)
     __syncwarp();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base), 0);
     if (elect_one()) {
-      const uint32_t idesc = int8_idesc(128, b_rows);
+      const uint32_t idesc = int8_idesc(128, mma_n);
       int s = 0;
       uint32_t phase = 0;
       bool good = true;
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(S_THREADS)
                 "{\n\t.reg .pred p;\n\t"
                 "setp.ne.b32 p, %4, 0;\n\t"
                 "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-                ::"r"(tmem + (uint32_t)(m * b_rows)), "l"(ad + (uint64_t)(m * 1024 + ks * 2)), "l"(bd + (uint64_t)(ks * 2)), "r"(idesc), "r"((kb > kb0 || ks > 0) ? 1u : 0u)
+                ::"r"(tmem + (uint32_t)(m * mma_n)), "l"(ad + (uint64_t)(m * 1024 + ks * 2)), "l"(bd + (uint64_t)(ks * 2)), "r"(idesc), "r"((kb > kb0 || ks > 0) ? 1u : 0u)
                 : "memory");
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(BAR(empty, s)) : "memory");
         if (++s == p.stages) { s = 0; phase ^= 1u; }
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(S_THREADS)
       const int t = m * 128 + row;
       for (int j = 16 * turn; j < b_rows; j += 32) {
         uint32_t v[16];
-        tmem_ld_16(lane_addr + (uint32_t)(m * b_rows + j), v);
+        tmem_ld_16(lane_addr + (uint32_t)(m * mma_n + j), v);
         const int seg = GATED && j >= p.width ? 1 : 0, c = (j - seg * p.width) / own, at = seg * own + j - seg * p.width - c * own;
         if (c != rank && t < p.M) {
           const int slot = rank < c ? rank : rank - 1;  // among the senders to c
@@ -543,11 +544,11 @@ __global__ void __launch_bounds__(S_THREADS)
     const int t = m * 128 + row;
     const float sa = t < p.M ? p.a_sf[t] : 0.f;
     for (int j = 16 * turn; j < own; j += 32) {
-      const int i0 = rank * own + j, n = n0 + i0;  // 16 columns; N is a multiple of 16
+      const int i0 = rank * own + j, n = n0 + i0;  // 16 columns, or the last 8 of the CTA's or of N
       if (n >= p.N) break;
       uint32_t v[16], u[16];
-      tmem_ld_16_async(lane_addr + (uint32_t)(m * b_rows + i0), v);
-      if (GATED) tmem_ld_16_async(lane_addr + (uint32_t)(m * b_rows + p.width + i0), u);
+      tmem_ld_16_async(lane_addr + (uint32_t)(m * mma_n + i0), v);
+      if (GATED) tmem_ld_16_async(lane_addr + (uint32_t)(m * mma_n + p.width + i0), u);
       tmem_ld_wait(v);
       if (GATED)
 #pragma unroll
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(S_THREADS)
       if (t < p.M && *abort_flag == 0) {
         uint4* to = reinterpret_cast<uint4*>(p.c + (size_t)t * p.ldc + n);
         to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        if (j + 8 < own && n + 8 < p.N) to[1] = make_uint4(o[4], o[5], o[6], o[7]);
       }
       __syncwarp();
     }
