@@ -285,6 +285,32 @@ def test_products_read_what_the_kernel_before_them_writes():
             assert torch.equal(ops.int8_matmul(a, b, a_sf, b_sf), want)
 
 
+@pytest.mark.parametrize("M", [1, 8, 40, 300, 257])
+def test_operands_that_other_kernels_write_right_before(M):
+    """B and its scales by kernels of another library, on the same stream, directly in front of the product."""
+    a, b, a_sf, b_sf = _operands(M, 2064, 1040, seed=1)
+    others = [_operands(M, 2064, 1040, seed=s) for s in (2, 3)]
+    wants = [ops.int8_matmul(*o) for o in others]
+    torch.cuda.synchronize()
+    for i in range(40):
+        for dst, src in zip((a, a_sf, b_sf, b), others[i % 2][:1] + others[i % 2][2:] + others[i % 2][1:2]):
+            dst.copy_(src)
+        assert torch.equal(ops.int8_matmul(a, b, a_sf, b_sf), wants[i % 2])
+
+
+def test_codes_of_a_norm_as_weights():
+    """What the norm casts may be B of the product right behind it as well."""
+    torch.manual_seed(5)
+    block, weight = torch.randn(512, 1024, device="cuda").half(), torch.ones(1024, device="cuda").half()
+    x, x_sf = ops.per_token_cast_int8(torch.randn(3, 1024, device="cuda").half())
+    codes, sf, _ = ops.block_norm_cast_int8(block, None, weight)
+    torch.cuda.synchronize()
+    want = ops.int8_matmul(x, codes, x_sf, sf)
+    for _ in range(20):
+        c, s, _ = ops.block_norm_cast_int8(block, None, weight)
+        assert torch.equal(ops.int8_matmul(x, c, x_sf, s), want)
+
+
 def test_other_streams_and_captured_graphs():
     torch.manual_seed(2)
     layer = Int8Linear(torch.bfloat16, 1024, 2048).cuda()

@@ -55,7 +55,9 @@ class Int8Linear(nn.Module):
         w = weight.detach().to(device=dev)
         if w.dtype not in (torch.float16, torch.bfloat16):
             w = w.to(self.act_torch_dtype)
-        codes, scales = ops.per_token_cast_int8(w if w.stride(-1) == 1 else w.contiguous())
+        if w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16:
+            w = w.clone(memory_format=torch.contiguous_format)
+        codes, scales = ops.per_token_cast_int8(w)
         with torch.no_grad():
             self.weight.copy_(codes)
             self.scales.copy_(scales)
