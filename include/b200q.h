@@ -329,7 +329,6 @@ typedef struct b200q_igemm_plan {
   int32_t cluster; /* kernel 2: CTAs that share the K of their columns, 1 .. 8 */
   int32_t stages;  /* kernel 2: ring slots of 128 bytes of K, 1 .. 16 */
   int32_t ctas;    /* kernel 1: CTAs, even; kernel 3: CTAs; kernel 2: output only */
-  int32_t tail_rows; /* kernel 1: up to 16 last rows that kernel 3 takes in a second launch; else 0 */
 } b200q_igemm_plan_t;
 int b200q_per_token_cast_int(const void* x, int ldx, void* out, int ldo, float* out_sf, int tokens, int hidden,
                              int act_dtype, void* stream);

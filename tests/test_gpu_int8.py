@@ -128,15 +128,14 @@ def test_every_plan_gives_the_same_bits(M, N, K, gated):
     """The sums being exact, neither the kernel nor the split of K changes a result."""
     a, b, a_sf, b_sf = _operands(M, N * (2 if gated else 1), K, seed=5)
     first = None
-    edits = [dict(kernel=1, width=w, ctas=c, tail_rows=0) for w, c in ((256, 2), (256, 6), (128, 4), (128, 148))]
-    edits += [dict(kernel=1, width=w, ctas=4, tail_rows=t) for w in (256, 128) for t in (1, 5, 16) if t < M]
+    edits = [dict(kernel=1, width=w, ctas=c) for w, c in ((256, 2), (256, 6), (128, 4), (128, 148))]
     if M <= 256:
-        edits += [dict(kernel=2, tail_rows=0, width=w * c, cluster=c, stages=s)
+        edits += [dict(kernel=2, width=w * c, cluster=c, stages=s)
                   for w, c, s in ((16, 1, 1), (48, 1, 3), (24, 1, 2), (56, 1, 2), (120, 1, 2), (80, 1, 3), (128, 1, 2), (16, 2, 4), (64, 2, 1), (16, 3, 2), (32, 4, 3),
                                   (16, 5, 5), (16, 7, 2), (16, 8, 4), (16, 1, 16))
                   if c <= -(-K // 128) and (M <= 64 or c < 5 and s < 16)]  # (what shared memory holds)
     if M <= 16:
-        edits += [dict(kernel=3, tail_rows=0, ctas=c) for c in (1, 3, 300)]
+        edits += [dict(kernel=3, ctas=c) for c in (1, 3, 300)]
     for edit in edits:
         out = torch.full((M, N), float("nan"), dtype=torch.float16, device="cuda")
         assert _planned(a, b, a_sf, b_sf, out, gated, **edit) == _lib.ST_OK, edit
@@ -148,19 +147,18 @@ def test_every_plan_gives_the_same_bits(M, N, K, gated):
 def test_plans_that_cannot_run_are_refused():
     a, b, a_sf, b_sf = _operands(8, 256, 512)
     out = torch.empty(8, 256, dtype=torch.float16, device="cuda")
-    good = {1: dict(kernel=1, width=256, ctas=2, tail_rows=0), 2: dict(kernel=2, width=64, cluster=2, stages=2, tail_rows=0),
-            3: dict(kernel=3, ctas=16, tail_rows=0)}
+    good = {1: dict(kernel=1, width=256, ctas=2), 2: dict(kernel=2, width=64, cluster=2, stages=2),
+            3: dict(kernel=3, ctas=16)}
     for edit in good.values():
         assert _planned(a, b, a_sf, b_sf, out, False, **edit) == _lib.ST_OK
     for kernel, edit in ((1, dict(kernel=0)), (1, dict(kernel=4)), (1, dict(width=64)), (1, dict(ctas=3)), (1, dict(ctas=0)),
-                         (1, dict(ctas=4096)), (1, dict(tail_rows=8)), (1, dict(tail_rows=-1)), (2, dict(cluster=9)),
+                         (1, dict(ctas=4096)), (2, dict(cluster=9)),
                          (2, dict(cluster=5)), (2, dict(cluster=0)), (2, dict(stages=0)), (2, dict(stages=17)), (2, dict(width=72)), (2, dict(cluster=1, width=60)),
-                         (2, dict(width=48)), (2, dict(width=512)), (2, dict(tail_rows=1)), (3, dict(ctas=0)), (3, dict(tail_rows=1))):
+                         (2, dict(width=48)), (2, dict(width=512)), (3, dict(ctas=0))):
         assert _planned(a, b, a_sf, b_sf, out, False, **{**good[kernel], **edit}) == _lib.ST_UNSUPPORTED, edit
     a, b, a_sf, b_sf = _operands(17, 256, 512)
     out = torch.empty(17, 256, dtype=torch.float16, device="cuda")
     assert _planned(a, b, a_sf, b_sf, out, False, **good[3]) == _lib.ST_UNSUPPORTED
-    assert _planned(a, b, a_sf, b_sf, out, False, **{**good[1], "tail_rows": 17}) == _lib.ST_UNSUPPORTED
 
 
 @pytest.mark.parametrize("M", [3, 300])

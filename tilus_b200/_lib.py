@@ -65,7 +65,7 @@ class Plan(ctypes.Structure):
 
 class IgemmPlan(ctypes.Structure):
     """b200q_igemm_plan_t of include/b200q.h."""
-    _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "rows", "width", "cluster", "stages", "ctas", "tail_rows")]
+    _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "rows", "width", "cluster", "stages", "ctas")]
 
     def as_dict(self):
         return {n: int(getattr(self, n)) for n, _ in self._fields_}

@@ -23,7 +23,6 @@ struct Int8Params {
   int rows, width;             // stream kernel: rows of A rounded up to 16, output columns of a CTA (or of a cluster)
   int cluster, stages;         // CTAs that share K, ring slots
   int early;                   // stream and row kernels: the kernel before this one does not write B
-  int beside;                  // row kernel: the kernel before this one computes the rows before its own, from the same operands
 };
 
 // api.cu

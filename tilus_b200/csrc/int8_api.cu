@@ -86,17 +86,15 @@ static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) 
   const int kblocks = igemm_kblocks(K);
   *pl = b200q_igemm_plan_t();
   double best = 1e30;
-  // Up to 16 rows past the last whole tile may go to the row kernel, beside the pair kernel's last round.
-  const int past = M > 256 && M % 256 <= 16 ? M % 256 : 0;
-  for (int cols = 256; cols >= 128; cols -= 128)
-    for (int tail = 0; tail <= past; tail += past > 0 ? past : 1) {
-      const int tiles = pair_tiles(M - tail, N, gated, cols), items = N / (gated ? 8 : 16), sms = di.sm_count;
-      double cost = pair_cost(tiles, gated, cols, kblocks, (double)(gated ? 2 : 1) * N * K, di);
-      if (tail > 0) cost += 0.7 * row_cost(tail, (double)(gated ? 2 : 1) * N * K, (items + 2 * sms - 1) / (2 * sms), K);
-      if (cost >= best) continue;
-      best = cost;
-      *pl = {1, 256, cols, 2, cols == 256 ? 6 : 8, 2 * (tiles < sms / 2 ? tiles : sms / 2), tail};
-    }
+  // (A last row tile of a few rows costs as much as any, but no more than that: 4097 x 12288 x 4096 takes 137.7 us, 4096 rows 132.5, and
+  // 4096 rows with the last one in a kernel of its own beside them 142.2.)
+  for (int cols = 256; cols >= 128; cols -= 128) {
+    const int tiles = pair_tiles(M, N, gated, cols);
+    const double cost = pair_cost(tiles, gated, cols, kblocks, (double)(gated ? 2 : 1) * N * K, di);
+    if (cost >= best) continue;
+    best = cost;
+    *pl = {1, 256, cols, 2, cols == 256 ? 6 : 8, 2 * (tiles < di.sm_count / 2 ? tiles : di.sm_count / 2)};
+  }
   if (M > kStreamRows) return;
   for (int s = 1; s <= 8 && 4 * (s - 1) <= kblocks; s *= 2)
     for (int per = s == 1 && kblocks >= 16 ? 2 : 1; per >= 1; --per) {
@@ -111,12 +109,12 @@ static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) 
       if (per == 1 && stages < (kblocks <= 8 * s ? 3 : 8)) stages = stream_stages(M, b_rows, s, di.max_smem);
       if (stages < (per == 1 ? 2 : 4)) continue;
       best = cost;
-      *pl = {2, (M + 15) / 16 * 16, width, s, stages, ctas, 0};
+      *pl = {2, (M + 15) / 16 * 16, width, s, stages, ctas};
     }
   if (M <= 16) {
     const int items = N / (gated ? 8 : 16);
     const double cost = row_cost(M, (double)(gated ? 2 : 1) * N * K, (items + 2 * di.sm_count - 1) / (2 * di.sm_count), K);
-    if (cost < best) *pl = {3, M, gated ? 8 : 16, 1, 1, items < 2 * di.sm_count ? items : 2 * di.sm_count, 0};
+    if (cost < best) *pl = {3, M, gated ? 8 : 16, 1, 1, items < 2 * di.sm_count ? items : 2 * di.sm_count};
   }
 }
 
@@ -165,17 +163,16 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
     e = int8_row_launch(p, gated, pl.ctas, stream);
   } else if (pl.kernel == 1) {
     const int pc = pl.width;
-    p.M = M - pl.tail_rows;
-    st = encode_rows(enc, &ta, a, K, p.M, lda, 128);
+    st = encode_rows(enc, &ta, a, K, M, lda, 128);
     if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, pc / 2);
     if (st != ST_OK) return st;
-    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)p.M};
+    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
     const cuuint64_t strides[1] = {(cuuint64_t)ldc * 2};
     const cuuint32_t box[2] = {64u, 32u}, steps[2] = {1u, 1u};
     const CUresult r = enc(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, c, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return cuda_failed((int)r);
-    p.m_tiles = (int)(((long long)p.M + 255) / 256);
+    p.m_tiles = (int)(((long long)M + 255) / 256);
     const int per = gated ? pc / 2 : pc;
     p.n_tiles = (N + per - 1) / per;
     if ((long long)p.m_tiles * p.n_tiles > 0x7fffffffll) return ST_UNSUPPORTED;
@@ -184,15 +181,6 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
     const long long fit = (32ll << 20) / (256ll * K);
     p.m_group = (int)(fit < 1 ? 1 : fit > p.m_tiles ? p.m_tiles : fit);
     e = int8_pair_launch(p, gated, pc, ta, tb, tc, pl.ctas, stream);
-    if (e == cudaSuccess && pl.tail_rows > 0) {
-      p.a += (size_t)p.M * lda;
-      p.a_sf += p.M;
-      p.c += (size_t)p.M * ldc;
-      p.M = pl.tail_rows;
-      p.beside = 1;
-      const int items = N / (gated ? 8 : 16), most = 2 * device_info().sm_count;
-      e = int8_row_launch(p, gated, items < most ? items : most, stream);
-    }
   } else {
     st = encode_rows(enc, &ta, a, K, M, lda, pl.rows);
     if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, pl.width);
@@ -209,11 +197,9 @@ static bool igemm_plan_ok(int M, int N, int K, bool gated, b200q_igemm_plan_t* p
   const DeviceInfo di = device_info();
   if (pl->kernel == 1) {
     if (pl->width != 128 && pl->width != 256) return false;
-    if (pl->tail_rows < 0 || pl->tail_rows > 16 || pl->tail_rows >= M) return false;
     if (pl->ctas < 2 || pl->ctas % 2 != 0 || pl->ctas > di.sm_count) return false;
     return int8_pair_smem_bytes(pl->width) <= di.max_smem;
   }
-  if (pl->tail_rows != 0) return false;
   if (pl->kernel == 3) return M <= 16 && pl->ctas >= 1 && pl->ctas <= 8 * di.sm_count;
   if (pl->kernel != 2 || M > kStreamRows) return false;
   pl->rows = (M + 15) / 16 * 16;

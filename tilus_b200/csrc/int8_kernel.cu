@@ -639,12 +639,10 @@ __global__ void __launch_bounds__(R_WARPS * 32, 2) int8_row_kernel(const Int8Par
     }
   };
   int item = blockIdx.x, buf = 0;
-  if ((p.early || p.beside) && item < items) load_b(item, k_lane);
-  if (!p.beside) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (!p.early && item < items) load_b(item, k_lane);
-  }
+  if (p.early && item < items) load_b(item, k_lane);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!p.early && item < items) load_b(item, k_lane);
   for (; item < items; item += gridDim.x, buf ^= 1) {
     int d[NT][4];
 #pragma unroll
@@ -693,9 +691,6 @@ __global__ void __launch_bounds__(R_WARPS * 32, 2) int8_row_kernel(const Int8Par
       p.c[(size_t)t * p.ldc + n] = (unsigned short)(pack_act(p.act, o, 0.f) & 0xffffu);
     }
   }
-  // Beside the pair kernel of the same call, whose last rows these are, it ran on the SMs that had no tile left: all it reads was there
-  // before that kernel's own wait.  The kernels behind wait for this one, so that it ends after the other.
-  if (p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------
