@@ -30,7 +30,7 @@ def test_plans():
                         continue
                     assert p["kernel"] == 2 and m <= 256 and p["rows"] == -(-m // 16) * 16 and 2 <= p["stages"] <= 16
                     assert p["cluster"] in (1, 2, 4, 8) and p["cluster"] <= -(-k // 128)
-                    assert p["width"] % (8 if p["cluster"] == 1 else 16 * p["cluster"]) == 0 and 16 <= p["width"] <= (128 if gated else 256)
+                    assert p["width"] % (8 * p["cluster"]) == 0 and 16 <= p["width"] <= (128 if gated else 256)
                     assert p["ctas"] == -(-n // p["width"]) * p["cluster"]
     for m, n, k in ((1, 24, 128), (1, 128, 24), (1, 16, 131072)):
         with pytest.raises(_lib.B200QError) as e:

@@ -27,8 +27,8 @@ static int pair_tiles(int M, int N, bool gated, int cols) {
   return (int)(((long long)M + 255) / 256 * ((N + per - 1) / per));
 }
 // Output columns of a stream kernel's tile with `s` CTAs to a cluster: an equal share of N for all SMs in as few rounds as the
-// tensor core's 256 columns allow, in units of 8, or of 16 for each CTA of a cluster.
-static int stream_unit(int s) { return s == 1 ? 8 : 16 * s; }
+// tensor core's 256 columns allow, in units of 8 for each CTA of a cluster.
+static int stream_unit(int s) { return 8 * s; }
 static int stream_width(int N, bool gated, int s, int sms) {
   const int unit = stream_unit(s), most = (gated ? 128 : 256) / unit * unit, groups = sms / s;
   const int rounds = (N + most * groups - 1) / (most * groups);
@@ -63,9 +63,10 @@ static double stream_cost(int M, int b_rows, int ctas, int s, int per, int kbloc
   const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, slots = per * di.sm_count, rounds = (ctas + slots - 1) / slots;
   const int busy = ctas < slots ? ctas : slots;
   const double tensor = per * accs * (128 + b_rows) * 1.05e-3, in = per * (rows + b_rows) * 1.05e-3;
-  const double memory = 128.0 * b_rows * busy / kHbm * (per == 1 ? 1.08 : 1.03);
+  const int sms = busy < 0.95 * di.sm_count ? (int)(0.95 * di.sm_count) : busy;  // an SM alone gets no more of the memory's rate
+  const double memory = 128.0 * b_rows * sms / kHbm * (per == 1 ? 1.08 : 1.03);
   const double piece = tensor > in ? (tensor > memory ? tensor : memory) : (in > memory ? in : memory);
-  return (per == 1 ? 2.8 : 2.6) + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.25 * s + 0.012 * s * M : 0.0) +
+  return (per == 1 ? 2.8 : 2.6) + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.25 * s + 0.012 * s * M * busy / slots : 0.0) +
          0.004 * per * M;
 }
 

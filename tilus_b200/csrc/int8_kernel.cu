@@ -371,7 +371,7 @@ static __host__ __device__ int stream_ring_bytes(int rows, int b_rows, int stage
 constexpr int S_INBOX_APART = 16384;
 static __host__ __device__ int stream_inbox_pitch(int b_rows, int cluster) { return b_rows / cluster * 4 + 16; }
 static __host__ __device__ int stream_inbox_bytes(int M, int b_rows, int cluster) {
-  return (cluster - 1) * M * stream_inbox_pitch(b_rows, cluster);
+  return cluster > 1 ? (cluster - 1) * M * stream_inbox_pitch(b_rows, cluster) + 64 : 0;  // (sums are read 16 at a time)
 }
 int int8_stream_smem_bytes(int M, int b_rows, int cluster, int stages) {
   const int inbox = stream_inbox_bytes(M, b_rows, cluster), ring = stream_ring_bytes((M + 15) / 16 * 16, b_rows, stages);
@@ -520,15 +520,18 @@ __global__ void __launch_bounds__(S_THREADS)
     for (int m = 0; m < accs; ++m) {
       if (m * 128 + (warp & 3) * 32 >= p.M) break;
       const int t = m * 128 + row;
-      for (int j = 16 * turn; j < b_rows; j += 32) {
-        uint32_t v[16];
-        tmem_ld_16(lane_addr + (uint32_t)(m * mma_n + j), v);
+      for (int j = 8 * turn; j < b_rows; j += 16) {
+        uint32_t v[8];
+        tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + j), v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i]));  // no use of v moves above the wait
         const int seg = GATED && j >= p.width ? 1 : 0, c = (j - seg * p.width) / own, at = seg * own + j - seg * p.width - c * own;
         if (c != rank && t < p.M) {
           const int slot = rank < c ? rank : rank - 1;  // among the senders to c
           const uint32_t to = map_to(inbox + (uint32_t)((slot * p.M + t) * pitch + at * 4), (uint32_t)c);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
             asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)(q * 16)), "r"(v[4 * q]),
                          "r"(v[4 * q + 1]), "r"(v[4 * q + 2]), "r"(v[4 * q + 3]) : "memory");
         }
