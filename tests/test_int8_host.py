@@ -20,7 +20,7 @@ def test_plans():
     for gated in (False, True):
         for m in (1, 8, 9, 16, 17, 64, 65, 200, 256, 257, 272, 273, 4096, 4097, 4113, 100000):
             for n in (16, 1040, 4096, 11008, 28672, 151936):
-                for k in (16, 144, 4096, 14336, 131056):
+                for k in (16, 144, 4096, 4112, 14336, 131056):
                     p = ops.int8_plan(m, n, k, gated)
                     if p["kernel"] == 1:
                         assert p["width"] in (128, 256) and p["ctas"] % 2 == 0 and 2 <= p["ctas"] <= 148
@@ -93,7 +93,8 @@ def test_cpu_tensors_are_refused(lib):
     w = torch.ones(64, dtype=torch.float16)
     for call in (lambda: ops.per_token_cast_int8(x), lambda: ops.int8_matmul(a, a, sf, sf), lambda: ops.int8_gate_up(a, a, sf, sf),
                  lambda: ops.block_norm(x, x, w), lambda: ops.block_norm_cast_int8(x, None, w),
-                 lambda: ops.block_norm_backward(x, None, x, x, w)):
+                 lambda: ops.block_norm_backward(x, None, x, x, w), lambda: BlockNorm("float16", 64)(x, None),
+                 lambda: Int8Linear("float16", 64, 32)(x)):
         with pytest.raises(ValueError, match="no CPU path"):
             call()
     with pytest.raises(TypeError):

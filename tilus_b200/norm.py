@@ -47,7 +47,7 @@ def block_norm(block, residual, weight, *, post_weight=None, gate=None, residual
     bookkeeping outlives a capture; capture ops.block_norm and ops.block_norm_backward instead."""
     operands = (block, residual, weight, post_weight, gate)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
-        if torch.cuda.is_current_stream_capturing():
+        if block.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("block_norm records gradients and cannot be captured: capture ops.block_norm and "
                                "ops.block_norm_backward, or capture under torch.no_grad()")
         return _BlockNorm.apply(*operands, residual_scale, eps)
