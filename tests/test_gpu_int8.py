@@ -123,7 +123,7 @@ def _planned(a, b, a_sf, b_sf, out, gated, **edit):
 
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("M,N,K", [(1, 272, 2064), (13, 48, 16), (40, 400, 1040), (130, 144, 304), (200, 272, 1040), (256, 80, 2048),
-                                   (261, 144, 2064), (528, 272, 400)])
+                                   (256, 16, 1040), (261, 144, 2064), (528, 272, 400)])
 def test_every_plan_gives_the_same_bits(M, N, K, gated):
     """The sums being exact, neither the kernel nor the split of K changes a result."""
     a, b, a_sf, b_sf = _operands(M, N * (2 if gated else 1), K, seed=5)
@@ -307,6 +307,30 @@ def test_codes_of_a_norm_as_weights():
     for _ in range(20):
         c, s, _ = ops.block_norm_cast_int8(block, None, weight)
         assert torch.equal(ops.int8_matmul(x, c, x_sf, s), want)
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_weights_cast_on_another_stream_of_a_captured_graph(M):
+    """A graph of two joined streams: one casts the weights, the other the activations, and multiplies."""
+    torch.manual_seed(3)
+    w, x = torch.randn(4096, 2048, device="cuda").half(), torch.randn(M, 2048, device="cuda").half()
+    want = ops.int8_matmul(*[t for pair in zip(ops.per_token_cast_int8(x), ops.per_token_cast_int8(w)) for t in pair])
+    static_w, static_x = torch.zeros_like(w), torch.zeros_like(x)
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            wc, wsf = ops.per_token_cast_int8(static_w)
+        xc, xsf = ops.per_token_cast_int8(static_x)
+        torch.cuda.current_stream().wait_stream(side)
+        out = ops.int8_matmul(xc, wc, xsf, wsf)
+    for sign in (1, -1, 1, -1):  # each replay has to see its own weights
+        static_w.copy_(w * sign)
+        static_x.copy_(x)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want * sign)
 
 
 def test_other_streams_and_captured_graphs():

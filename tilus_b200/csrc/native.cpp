@@ -426,8 +426,9 @@ bool optional_tensor(PyObject* o, const char* name, const at::Tensor** t) {
 
 // A product may read its operand B (weights) before the kernel in front of it has ended, unless that one writes it.  What writes
 // int8 codes here are the casts, and each kernel of these operators lets the next one start only when the one before itself has
-// ended: so it is the stream's latest cast that matters.  Its outputs are noted until a product has been launched behind it (which
-// waits for it and for everything before).
+// ended: so it is a stream's latest cast that matters.  Its outputs are noted until a product has been launched behind it (which
+// waits for it and for everything before).  Other streams' latest casts count too: in a capture that joins streams the product's edge
+// from each kernel that it follows may be one that lets it set up early.
 void codes_written(int device, cudaStream_t stream, const void* codes, int64_t bytes) {
   std::lock_guard<std::mutex> lock(g_mutex);
   StreamBuffers& b = buffers_of(device, stream);
@@ -436,10 +437,12 @@ void codes_written(int device, cudaStream_t stream, const void* codes, int64_t b
 }
 bool settled(int device, cudaStream_t stream, const void* operand, int64_t bytes) {
   std::lock_guard<std::mutex> lock(g_mutex);
-  StreamBuffers& b = buffers_of(device, stream);
   const char* p = static_cast<const char*>(operand);
-  const bool apart = b.cast_begin == nullptr || p >= b.cast_end || p + bytes <= b.cast_begin;
-  b.cast_begin = b.cast_end = nullptr;
+  bool apart = true;
+  for (const auto& b : pool()) {
+    if (b->device == device && b->cast_begin && p < b->cast_end && p + bytes > b->cast_begin) apart = false;
+    if (b->device == device && b->stream == stream) b->cast_begin = b->cast_end = nullptr;
+  }
   return apart;
 }
 
