@@ -1,4 +1,4 @@
-// Parameter blocks of the 8-bit integer products (int8_kernel.cu) and of the host code that they share with api.cu.
+// Parameter blocks of the 8-bit integer products (int8_kernel.cu) and of the host code (int8_api.cu), and what that shares with api.cu.
 #pragma once
 #include <cuda.h>
 
@@ -21,7 +21,7 @@ struct Int8Params {
   float clamp;
   int tiles, m_tiles, n_tiles, m_group;  // pair kernel: output tiles and their raster groups
   int rows, width;             // stream kernel: rows of A rounded up to 16, output columns of a CTA (or of a cluster)
-  int cluster, stages;         // CTAs that share K, ring slots
+  int cluster, stages, smem;   // CTAs that share K, ring slots, dynamic shared memory
   int early;                   // stream and row kernels: the kernel before this one does not write B
 };
 

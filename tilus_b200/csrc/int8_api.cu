@@ -36,7 +36,7 @@ static int stream_width(int N, bool gated, int s, int sms) {
   return width < 16 ? 16 : width;
 }
 static int stream_stages(int M, int b_rows, int s, int budget) {
-  int stages = 16;
+  int stages = 12;  // (with 16 64 x 1024 x 8192 takes 7.3 us, not 7.0)
   while (stages > 1 && int8_stream_smem_bytes(M, b_rows, s, stages) > budget) --stages;
   return stages;
 }
@@ -55,18 +55,23 @@ static double row_cost(int M, double b_bytes, int rounds, int K) {
   return memory > latency ? memory : latency;
 }
 
-// A piece of 128 bytes of K takes what the slowest of three takes: reading B, bringing both operands' rows to the SM (121 GB/s a SM),
+// Rows that start between two 32-byte sectors: their pieces of 128 bytes come in one sector more, of two lines.  (K = 4096 / 4128 / 4112, us:
+// 1024 x 18944 50 / 53 / 65, 200 x 4736 12.9 / 14.1 / 19.7.)
+static bool split_sectors(int K) { return K % 32 != 0; }
+
+// A piece of 128 bytes of K takes what the slowest of three takes: reading B, bringing both operands' rows to the SM (121 GB/s a SM, or half of that),
 // and the tensor core's reading them (about as fast, but whole accumulators' rows of A).  A cluster's exchange goes by its size
 // and rows: 64 x 4096 x 14336 takes 20.1 us alone, 14.5 in pairs, 15.3 in fours; 128 rows 20.7, 17.1, 19.4.  Two CTAs to an SM
 // (`per` 2) share it, but one starts and ends under the other: 8 x 28672 gated 22.5 us with one, 20.6 with two.
-static double stream_cost(int M, int b_rows, int ctas, int s, int per, int kblocks, const DeviceInfo& di) {
+static double stream_cost(int M, int b_rows, int ctas, int s, int per, int K, const DeviceInfo& di) {
+  const int kblocks = igemm_kblocks(K);
   const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, slots = per * di.sm_count, rounds = (ctas + slots - 1) / slots;
   const int busy = ctas < slots ? ctas : slots;
-  const double tensor = per * accs * (128 + b_rows) * 1.05e-3, in = per * (rows + b_rows) * 1.05e-3;
+  const double tensor = per * accs * (128 + b_rows) * 1.05e-3, in = per * (rows + b_rows) * (split_sectors(K) ? 2.1e-3 : 1.05e-3);
   const int sms = busy < 0.95 * di.sm_count ? (int)(0.95 * di.sm_count) : busy;  // an SM alone gets no more of the memory's rate
   const double memory = 128.0 * b_rows * sms / kHbm * (per == 1 ? 1.08 : 1.03);
   const double piece = tensor > in ? (tensor > memory ? tensor : memory) : (in > memory ? in : memory);
-  return (per == 1 ? 2.8 : 2.6) + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.25 * s + 0.012 * s * M * busy / slots : 0.0) +
+  return (per == 1 ? 2.8 : 2.6) + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.2 + 0.05 * s + 0.012 * s * M * busy / slots : 0.0) +
          0.004 * per * M;
 }
 
@@ -74,9 +79,10 @@ static double stream_cost(int M, int b_rows, int ctas, int s, int per, int kbloc
 // through the same SM.  A tile takes no less than its outputs do, 3.1 and 1.9 us (gated 2.6: half
 // of the writers have none of a narrow tile).  Up front, and for the last tile's outputs: 5.6 and 3.9.  And
 // B has to be read.
-static double pair_cost(int tiles, bool gated, int cols, int kblocks, double b_bytes, const DeviceInfo& di) {
+static double pair_cost(int tiles, bool gated, int cols, int K, double b_bytes, const DeviceInfo& di) {
   const int pairs = di.sm_count / 2, rounds = (tiles + pairs - 1) / pairs;
-  const double products = kblocks * (cols == 256 ? 0.30 : 0.195), outputs = cols == 256 ? 3.1 : gated ? 2.6 : 1.9;
+  const double piece = split_sectors(K) ? (cols == 256 ? 0.42 : 0.32) : cols == 256 ? 0.30 : 0.195;
+  const double products = igemm_kblocks(K) * piece, outputs = cols == 256 ? 3.1 : gated ? 2.6 : 1.9;
   const double start = cols == 256 ? 5.6 : 3.9, all = products + (rounds - 1) * (products > outputs ? products : outputs);
   const double memory = 1.15 * b_bytes / kHbm;
   return start + (all > memory ? all : memory);
@@ -91,7 +97,7 @@ static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) 
   // 4096 rows with the last one in a kernel of its own beside them 142.2.)
   for (int cols = 256; cols >= 128; cols -= 128) {
     const int tiles = pair_tiles(M, N, gated, cols);
-    const double cost = pair_cost(tiles, gated, cols, kblocks, (double)(gated ? 2 : 1) * N * K, di);
+    const double cost = pair_cost(tiles, gated, cols, K, (double)(gated ? 2 : 1) * N * K, di);
     if (cost >= best) continue;
     best = cost;
     *pl = {1, 256, cols, 2, cols == 256 ? 6 : 8, 2 * (tiles < di.sm_count / 2 ? tiles : di.sm_count / 2)};
@@ -101,14 +107,15 @@ static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) 
     for (int per = s == 1 && kblocks >= 16 ? 2 : 1; per >= 1; --per) {
       const int width = stream_width(N, gated, s, per * di.sm_count), b_rows = gated ? 2 * width : width;
       const int ctas = (N + width - 1) / width * s;
-      const double cost = stream_cost(M, b_rows, ctas, s, per, kblocks, di);
+      const double cost = stream_cost(M, b_rows, ctas, s, per, K, di);
       if (cost >= best) continue;
-      // half an SM's shared memory for one of two CTAs, or where that is depth enough for the length of K: a CTA of the stream's next
-      // launch has room next to it then (126 x 9376 x 704, us with 4 stages / 9 of a whole SM's: 4.6 / 5.4; 100 x 11008 x 4224 with 4 / 8:
-      // 14.0 / 11.5)
-      int stages = stream_stages(M, b_rows, s, 113 * 1024);
-      if (per == 1 && stages < (kblocks <= 8 * s ? 3 : 8)) stages = stream_stages(M, b_rows, s, di.max_smem);
-      if (stages < (per == 1 ? 2 : 4)) continue;
+      // Half an SM's shared memory for one of two CTAs, or where that is depth enough for the length of K: a CTA of the stream's next
+      // launch has room next to it then.  (us, K 1024 / 2048 / 4096, half an SM's stages / ten of a whole one's: 24 x 9472, 8 stages, 4.4
+      // 7.6 10.7 / 5.0 7.7 10.1; 100 x 9472, 4 stages, 5.4 8.6 12.8 / 5.6 8.0 10.5; 24 x 4736, 12 stages, 3.8 5.2 8.4 / 4.2 5.8 9.0.)
+      // A cluster has whole SMs in any case.
+      int stages = stream_stages(M, b_rows, s, s > 1 ? di.max_smem : 113 * 1024);
+      if (s == 1 && per == 1 && stages < 12 && (stages < 3 || 3 * kblocks > 8 * stages)) stages = stream_stages(M, b_rows, s, di.max_smem);
+      if (stages < (per == 1 ? 2 : 3)) continue;
       best = cost;
       *pl = {2, (M + 15) / 16 * 16, width, s, stages, ctas};
     }
@@ -187,6 +194,9 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
     if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, pl.width);
     if (st != ST_OK) return st;
     p.rows = pl.rows; p.width = pl.width; p.cluster = pl.cluster; p.stages = pl.stages;
+    // A cluster's CTAs have an SM each to themselves.  Next to one another, two clusters (of one launch or of two streams) could each
+    // hold the tensor memory that the other's second CTA waits for.
+    p.smem = pl.cluster > 1 ? device_info().max_smem : int8_stream_smem_bytes(M, gated ? 2 * pl.width : pl.width, 1, pl.stages);
     p.tiles = pl.ctas / pl.cluster;
     e = int8_stream_launch(p, gated, ta, tb, stream);
   }

@@ -11,16 +11,21 @@
 // Both operands are K-major as they come (rows of 128 bytes, 128-byte swizzle); TMA fills what lies behind the last row
 // or the end of K with zeros, so ragged sizes cost no code in the main loops.
 //
-// Two kernels:
+// Three kernels:
 //   pair    two CTAs per tile of 256 rows x 256 or 128 columns of the product (gated: the gate columns in one CTA's half of B and
 //           their partners in the other's), tcgen05.mma with cta_group::2, accumulators double-buffered in tensor memory so that a tile's
 //           epilogue runs under the next one's products.  For many rows: bound by the tensor cores.
 //   stream  up to 256 rows, all of them against an equal share of the columns in each CTA, so that B is read once: bound by that.
+//   row     up to 16 rows where the product is small: no pipeline to fill, mma.sync from registers.  Bound by the latency of its loads.
+// On a B200, between launches of a graph: pair, 4096 x 8192 x 8192, 162 us (3.40 POP/s, the tensor pipe busy 88 % of the time); 4096 x 28672
+// x 8192 gated 562 to 641 us as the power limit has it (3.0 to 3.4 POP/s); stream, 8 x 28672 x 4096 gated 20.6 us (5.7 TB/s), 1 x 16384 x
+// 8192 27 us, 64 x 28672 x 4096 gated 23 us; row, 1 x 4096 x 4096 4.1 us.
 //
-// Both are launched with programmatic stream serialization: they set up under the end of the kernel before them.  All they read
-// before that kernel has ended is, in the stream kernel and where the caller says that it may (`early`), rows of B.  Like the
+// All are launched with programmatic stream serialization: they set up under the end of the kernel before them.  All they read
+// before that kernel has ended is, in the stream and row kernels and where the caller says that it may (`early`), rows of B.  Like the
 // row-wise kernels they let the kernel behind them start only after their own wait, so that whatever runs then, the kernel
-// before the last has ended.
+// before the last has ended; and only once they have their tensor memory, which a CTA behind them, waiting for their end, could
+// otherwise hold.
 #include "int8.cuh"
 #include "umma_common.cuh"
 
@@ -386,10 +391,6 @@ __device__ __forceinline__ void stream_load_b(const Int8Params& p, const CUtenso
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(dst + (uint32_t)(h * p.width) * 128u), "l"(tb), "r"(bar), "r"(kb * 128), "r"(n0 + h * p.N) : "memory");
 }
-__device__ __forceinline__ void tmem_ld_16_async(uint32_t taddr, uint32_t* v) {
-  tmem_ld_8_async(taddr, v);
-  tmem_ld_8_async(taddr + 8u, v + 8);
-}
 
 template <bool GATED>
 __global__ void __launch_bounds__(S_THREADS)
@@ -416,10 +417,14 @@ __global__ void __launch_bounds__(S_THREADS)
   const bool apart = stream_inbox_bytes(p.M, b_rows, S) <= S_INBOX_APART;
   const uint32_t inbox = apart ? ring + (uint32_t)stream_ring_bytes(p.rows, b_rows, p.stages) : ring;
 
-  if (tid == 0) {
-    for (int i = 0; i < p.stages; ++i) { mbar_init(BAR(full, i), 1); mbar_init(BAR(empty, i), 1); }
-    mbar_init(BAR(done, 0), 1);
-    bars->abort_flag = 0;
+  if (tid <= p.stages) {
+    if (tid < p.stages) {
+      mbar_init(BAR(full, tid), 1);
+      mbar_init(BAR(empty, tid), 1);
+    } else {
+      mbar_init(BAR(done, 0), 1);
+      bars->abort_flag = 0;
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -468,6 +473,8 @@ __global__ void __launch_bounds__(S_THREADS)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     __syncwarp();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base), 0);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (elect_one()) {
       const uint32_t idesc = int8_idesc(128, mma_n);
       int s = 0;
@@ -493,10 +500,8 @@ __global__ void __launch_bounds__(S_THREADS)
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(BAR(done, 0)) : "memory");
     }
     __syncwarp();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
   } else {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     for (int i = tid - 32 * (S_COPIERS + 1); i < b_rows; i += S_THREADS - 32 * (S_COPIERS + 1)) {
       const int n = n0 + (GATED ? i % p.width : i);
       bars->b_sf[i] = n < p.N ? p.b_sf[GATED && i >= p.width ? n + p.N : n] : 0.f;
@@ -549,9 +554,14 @@ __global__ void __launch_bounds__(S_THREADS)
     for (int j = 16 * turn; j < own; j += 32) {
       const int i0 = rank * own + j, n = n0 + i0;  // 16 columns, or the last 8 of the CTA's or of N
       if (n >= p.N) break;
-      uint32_t v[16], u[16];
-      tmem_ld_16_async(lane_addr + (uint32_t)(m * mma_n + i0), v);
-      if (GATED) tmem_ld_16_async(lane_addr + (uint32_t)(m * mma_n + p.width + i0), u);
+      const bool full = j + 8 < own;
+      uint32_t v[16] = {}, u[16] = {};
+      tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + i0), v);
+      if (full) tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + i0 + 8), v + 8);
+      if constexpr (GATED) {
+        tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + p.width + i0), u);
+        if (full) tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + p.width + i0 + 8), u + 8);
+      }
       tmem_ld_wait(v);
       if (GATED)
 #pragma unroll
@@ -584,7 +594,7 @@ __global__ void __launch_bounds__(S_THREADS)
       if (t < p.M && *abort_flag == 0) {
         uint4* to = reinterpret_cast<uint4*>(p.c + (size_t)t * p.ldc + n);
         to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        if (j + 8 < own && n + 8 < p.N) to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        if (full && n + 8 < p.N) to[1] = make_uint4(o[4], o[5], o[6], o[7]);
       }
       __syncwarp();
     }
@@ -732,8 +742,7 @@ static cudaError_t stream_launch(const Int8Params& p, const CUtensorMap& ta, con
   static std::atomic<bool> allowed[16];
   const cudaError_t e = allow_smem(int8_stream_kernel<GATED>, allowed);
   if (e != cudaSuccess) return e;
-  return launch_behind(int8_stream_kernel<GATED>, p.tiles * p.cluster, S_THREADS, p.cluster, int8_stream_smem_bytes(p.M, (GATED ? 2 : 1) * p.width, p.cluster, p.stages),
-                       stream, p, ta, tb);
+  return launch_behind(int8_stream_kernel<GATED>, p.tiles * p.cluster, S_THREADS, p.cluster, p.smem, stream, p, ta, tb);
 }
 
 cudaError_t int8_pair_launch(const Int8Params& p, bool gated, int cols, const CUtensorMap& ta, const CUtensorMap& tb,
