@@ -7,9 +7,7 @@ namespace b200q {
 constexpr int NORM_ROWS_FROM = 888;   // rows from which a block norm has its rows copied ahead (three to a CTA)
 constexpr int NORM_ROWS_STAGES = 4;   // rows in shared memory then
 constexpr int NORM_BACK_THREADS = 512;  // of an SM in the gradient's kernel, which takes up to 128 registers a thread
-
 constexpr int NORM_BACK_STAGES = 4;     // rows in shared memory
-constexpr int NORM_BACK_ROWS = 2;       // rows of a CTA at least, whose sums over them are as many bytes as six rows of a 16-bit type
 
 struct CastIntParams {
   const unsigned short* x;  // [T, D], row stride ldx, fp16 or bf16

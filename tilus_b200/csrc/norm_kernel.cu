@@ -782,38 +782,52 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
   }
 }
 
-// The sums of the CTAs' shares: 32 columns a CTA, eight runs of shares side by side, joined in order.  (With 32 runs to a CTA of 1024
-// threads 4096 x 4096 took 52.2 us, not 50.8.)  blockIdx.y: grad_weight, grad_post, then one for each gate.
-__global__ void __launch_bounds__(256) norm_sums_kernel(const NormBackwardParams p) {
-  __shared__ float part[8][33];
-  start_behind();
-  const int which = (int)blockIdx.y, col = (int)blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5;
-  const float* from = p.partial;
-  float* to = p.grad_weight;
-  int n = p.grid;
-  if (which == 1) {
-    if (!p.post) return;
-    from += (long long)p.grid * p.D;
-    to = p.grad_post;
-  } else if (which > 1) {
-    const int g = which - 2;
-    n = p.ctas_per_gate;
-    from += ((long long)2 * p.grid + (long long)g * n) * p.D;
-    to = p.grad_gate + (long long)g * p.D;
-  }
+// The sums of the CTAs' shares: 32 columns a CTA, 24 runs of shares side by side, joined in order.  A thread's loads, which come from L2,
+// are under way together: seven are a CTA to each SM.  (511 x 4096, us for the whole gradient: 8 runs and a loop unrolled ten times,
+// whose rest went one by one, 15.7; 8 runs in tens 14.4, 16 in tens 13.3, 24 in sevens 12.7.)  blockIdx.y: grad_weight, grad_post, then
+// gates, several to a CTA: the more there are the fewer shares each has.
+constexpr int SUMS_RUNS = 24, SUMS_BATCH = 7;
+static __host__ __device__ int sums_runs(int gates) { return gates < SUMS_RUNS ? SUMS_RUNS / gates : 1; }  // of a gate
+// `runs` of n rows of `from`, this thread's the run `part`
+__device__ __forceinline__ float sum_run(const float* from, int n, int part, int runs, long long D) {
   float s = 0.f;
-  if (col < p.D) {
-    const int i0 = n * run / 8, i1 = n * (run + 1) / 8;
-#pragma unroll 10
-    for (int i = i0; i < i1; ++i) s += from[(long long)i * p.D + col];
-  }
-  part[run][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (run == 0 && col < p.D) {
+  const int i1 = n * (part + 1) / runs;
+  for (int i = n * part / runs; i < i1; i += SUMS_BATCH) {
+    float x[SUMS_BATCH];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x & 31];
-    to[col] = s;
+    for (int j = 0; j < SUMS_BATCH; ++j) x[j] = i + j < i1 ? from[(i + j) * D] : 0.f;
+#pragma unroll
+    for (int j = 0; j < SUMS_BATCH; ++j) s += x[j];
   }
+  return s;
+}
+__global__ void __launch_bounds__(SUMS_RUNS * 32) norm_sums_kernel(const NormBackwardParams p) {
+  __shared__ float sums[SUMS_RUNS][33];
+  start_behind();
+  const int which = (int)blockIdx.y, lane = threadIdx.x & 31, col = (int)blockIdx.x * 32 + lane, run = threadIdx.x >> 5;
+  const bool there = col < p.D;
+  if (which <= 1) {
+    if (which == 1 && !p.post) return;
+    const float* from = p.partial + (long long)which * p.grid * p.D + col;
+    float s = there ? sum_run(from, p.grid, run, SUMS_RUNS, p.D) : 0.f;
+    sums[run][lane] = s;
+    __syncthreads();
+    if (run > 0 || !there) return;
+#pragma unroll
+    for (int i = 1; i < SUMS_RUNS; ++i) s += sums[i][lane];
+    (which == 0 ? p.grad_weight : p.grad_post)[col] = s;
+    return;
+  }
+  const int runs = sums_runs(p.gates), at = run / runs, part = run - at * runs;
+  const int g = (which - 2) * (SUMS_RUNS / runs) + at, n = p.ctas_per_gate;
+  const bool mine = there && at < SUMS_RUNS / runs && g < p.gates;
+  float s = mine ? sum_run(p.partial + ((long long)2 * p.grid + (long long)g * n) * p.D + col, n, part, runs, p.D) : 0.f;
+  sums[run][lane] = s;
+  __syncthreads();
+  if (part > 0 || !mine) return;
+#pragma unroll
+  for (int i = 1; i < SUMS_RUNS; ++i) s += i < runs ? sums[run + i < SUMS_RUNS ? run + i : 0][lane] : 0.f;
+  p.grad_gate[(long long)g * p.D + col] = s;
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------
@@ -916,8 +930,9 @@ static cudaError_t backward_type(const NormBackwardParams& p, cudaStream_t strea
     default: e = backward_rows<ACT, F32, 4>(p, stream); break;
   }
   if (e != cudaSuccess) return e;
-  const int sums = 2 + (p.grad_gate && p.ctas_per_gate > 1 ? p.gates : 0);
-  return launch_behind(norm_sums_kernel, dim3((unsigned)((p.D + 31) / 32), (unsigned)sums, 1), 256, 0, stream, p);
+  const int gates = SUMS_RUNS / sums_runs(p.gates);  // of a CTA
+  const int sums = 2 + (p.grad_gate && p.ctas_per_gate > 1 ? (p.gates + gates - 1) / gates : 0);
+  return launch_behind(norm_sums_kernel, dim3((unsigned)((p.D + 31) / 32), (unsigned)sums, 1), SUMS_RUNS * 32, 0, stream, p);
 }
 // The shape of the gradient's launch: threads and vectors of a row, CTAs (512 threads to an SM), and stages for the rows ahead.
 void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gate, int sms, int max_smem, NormBackwardParams* p) {
@@ -926,7 +941,10 @@ void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gat
   p->vectors = nvec <= (few ? 512 : 256) ? 1 : nvec <= 1024 ? 2 : 4;
   p->threads = ((nvec + p->vectors - 1) / p->vectors + 31) / 32 * 32;
   const int per_sm = NORM_BACK_THREADS / p->threads < 8 ? NORM_BACK_THREADS / p->threads : 8, most = sms * per_sm;
-  const int runs = (tokens_per_gate + NORM_BACK_ROWS - 1) / NORM_BACK_ROWS;  // that a gate's rows are enough for
+  // Runs that a gate's rows are enough for: a row each where the SMs are as many, else two, since a CTA's sums over rows are as many bytes
+  // as six rows.  (us, two rows each / one: 8 x 4096 9.3 / 7.9, 148 x 4096 10.3 / 8.9, 296 x 1024 7.4 / 7.7.)
+  const int single = sms / gates < tokens_per_gate ? sms / gates : tokens_per_gate, twos = (tokens_per_gate + 1) / 2;
+  const int runs = single > twos ? single : twos;
   if (gates >= most) {
     p->ctas_per_gate = 1;
     p->grid = most;
