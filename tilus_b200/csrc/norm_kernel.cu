@@ -937,7 +937,7 @@ static cudaError_t backward_type(const NormBackwardParams& p, cudaStream_t strea
 // The shape of the gradient's launch: threads and vectors of a row, CTAs (512 threads to an SM), and stages for the rows ahead.
 void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gate, int sms, int max_smem, NormBackwardParams* p) {
   const int nvec = D / 8;
-  const bool few = (long long)gates * tokens_per_gate <= 16ll * sms;
+  const bool few = (long long)gates * tokens_per_gate <= 12ll * sms;
   p->vectors = nvec <= (few ? 512 : 256) ? 1 : nvec <= 1024 ? 2 : 4;
   p->threads = ((nvec + p->vectors - 1) / p->vectors + 31) / 32 * 32;
   const int per_sm = NORM_BACK_THREADS / p->threads < 8 ? NORM_BACK_THREADS / p->threads : 8, most = sms * per_sm;
