@@ -144,7 +144,8 @@ def test_gradients(T, D, form):
     _check_gradients(s, 0.75)
 
 
-@pytest.mark.parametrize("T,gates,post", [(6, 2, True), (640, 640, False), (600, 300, True), (301, 7, True), (64, 2, False)])
+@pytest.mark.parametrize("T,gates,post", [(6, 2, True), (640, 640, False), (600, 300, True), (301, 7, True), (64, 2, False), (96, 24, True),
+                                          (120, 30, True), (75, 25, False)])
 def test_gradients_of_several_gates(T, gates, post):
     _check_gradients(_make(T, 264, torch.bfloat16, wide=True, post=post, gates=gates, grads=True), 1.0)
 

@@ -334,7 +334,7 @@ size_t b200q_block_norm_scratch_bytes(int tokens, int hidden, int gates) {
   NormBackwardParams p;
   const DeviceInfo di = device_info();
   norm_backward_shape(hidden, false, gates > 0 ? gates : 1, tokens / (gates > 0 ? gates : 1), di.sm_count, di.max_smem, &p);
-  return (size_t)3 * p.grid * hidden * sizeof(float);
+  return (size_t)2 * p.grid * hidden * sizeof(float);
 }
 
 int b200q_block_norm_backward(const b200q_block_norm_t* a, const void* grad_x, long long lddx, const void* grad_new, long long lddn,

@@ -38,10 +38,11 @@ struct NormBackwardParams {
   unsigned short* grad_block;
   void* grad_residual;              // null: not wanted
   float *grad_weight, *grad_post, *grad_gate;  // [D], [D], [gates, D] fp32
-  float* partial;                   // [CTAs][2 or 3][D]
+  float* partial;                   // [2][CTAs][D]: shares of grad_weight, and of grad_post or S
   int* status;                      // workspace status header
   int T, D, gates, tokens_per_gate;
   int ctas_per_gate, grid;          // CTAs that share a gate's rows; several gates to a CTA where it is 1
+  int sums_runs, sums_per, gate_per;  // runs of a gate's shares in the second kernel; 65536 / runs + 1; 65536 / ctas_per_gate + 1
   int threads, vectors, stages, smem;  // threads of a row, its vectors of a thread, rows in shared memory and their bytes
   long long ldb, ldr, ldg, lddx, lddn, lddb, lddr;
   float scale, eps;

@@ -729,23 +729,27 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
         if (me == 0) fetch();
       }
     }
-    // the gate's sums: its own gradient, and what its rows give post
+    // S: as it is where CTAs share the gate, whose sums the second kernel takes apart; else the gate's own gradient, and what its rows
+    // give post.
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int v = me + i * tpr;
       if (v >= nvec) continue;
+      const long long to = ((long long)p.grid + blockIdx.x) * p.D + v * 8;
+      if (p.ctas_per_gate > 1) {
+        if (p.post || p.grad_gate) Wide<ACT, true>::store(p.partial, to, S[i]);
+        continue;
+      }
       F2 x[4];
       if (p.grad_gate) {
-        float* to = p.ctas_per_gate == 1 ? p.grad_gate + (long long)g * p.D : p.partial + ((long long)2 * p.grid + blockIdx.x) * p.D;
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = both(1.f);
         if (p.post) load(p.post, i, x);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = x[k] * S[i][k];
-        Wide<ACT, true>::store(to, v * 8, x);
+        Wide<ACT, true>::store(p.grad_gate + (long long)g * p.D, v * 8, x);
       }
       if (p.post) {
-        const long long to = ((long long)p.grid + blockIdx.x) * p.D + v * 8;
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = both(1.f);
         if (p.gate) load(p.gate + g * p.ldg, i, x);
@@ -784,50 +788,81 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
 
 // The sums of the CTAs' shares: 32 columns a CTA, 24 runs of shares side by side, joined in order.  A thread's loads, which come from L2,
 // are under way together: seven are a CTA to each SM.  (511 x 4096, us for the whole gradient: 8 runs and a loop unrolled ten times,
-// whose rest went one by one, 15.7; 8 runs in tens 14.4, 16 in tens 13.3, 24 in sevens 12.7.)  blockIdx.y: grad_weight, grad_post, then
-// gates, several to a CTA: the more there are the fewer shares each has.
+// whose rest went one by one, 15.7; 8 runs in tens 14.4, 16 in tens 13.3, 24 in sevens 12.7.)  blockIdx.y: grad_weight, grad_post
+// and up to 24 gates, whose runs are the fewer the more they are; more gates after that.  (Quotients by products: several divisions of a
+// thread's cost 0.3 us.)
 constexpr int SUMS_RUNS = 24, SUMS_BATCH = 7;
-static __host__ __device__ int sums_runs(int gates) { return gates < SUMS_RUNS ? SUMS_RUNS / gates : 1; }  // of a gate
-// `runs` of n rows of `from`, this thread's the run `part`
-__device__ __forceinline__ float sum_run(const float* from, int n, int part, int runs, long long D) {
+// Run `part` of n shares at `from`, `factor(share)` in front of each.  The runs meet at n * part / (runs), taken as a product with `per` =
+// 65536 / runs + 1 (up to a few thousand shares the last one ends at n: the product is too large by less than one).
+template <class Factor>
+__device__ __forceinline__ float sum_run(const float* from, int n, int part, int per, long long D, Factor factor) {
   float s = 0.f;
-  const int i1 = n * (part + 1) / runs;
-  for (int i = n * part / runs; i < i1; i += SUMS_BATCH) {
+  const int i1 = (int)((unsigned)(n * (part + 1)) * (unsigned)per >> 16);
+  for (int i = (int)((unsigned)(n * part) * (unsigned)per >> 16); i < i1; i += SUMS_BATCH) {
     float x[SUMS_BATCH];
 #pragma unroll
-    for (int j = 0; j < SUMS_BATCH; ++j) x[j] = i + j < i1 ? from[(i + j) * D] : 0.f;
+    for (int j = 0; j < SUMS_BATCH; ++j) x[j] = i + j < i1 ? from[(i + j) * D] * factor(i + j) : 0.f;
 #pragma unroll
     for (int j = 0; j < SUMS_BATCH; ++j) s += x[j];
   }
   return s;
 }
-__global__ void __launch_bounds__(SUMS_RUNS * 32) norm_sums_kernel(const NormBackwardParams p) {
+// GATES: 0 one gate, none or CTAs that leave nothing for several to be done; else CTAs share several gates, 1 up to 24, 2 more.
+template <int ACT, int GATES>
+__global__ void __launch_bounds__(SUMS_RUNS * 32, 2) norm_sums_kernel(const NormBackwardParams p) {
   __shared__ float sums[SUMS_RUNS][33];
   start_behind();
   const int which = (int)blockIdx.y, lane = threadIdx.x & 31, col = (int)blockIdx.x * 32 + lane, run = threadIdx.x >> 5;
   const bool there = col < p.D;
-  if (which <= 1) {
-    if (which == 1 && !p.post) return;
-    const float* from = p.partial + (long long)which * p.grid * p.D + col;
-    float s = there ? sum_run(from, p.grid, run, SUMS_RUNS, p.D) : 0.f;
+  auto value = [&](const unsigned short* from) {
+    return ACT == 0 ? __half2float(__ushort_as_half(from[col])) : __uint_as_float((uint32_t)from[col] << 16);
+  };
+  const auto one = [](int) { return 1.f; };
+  constexpr int PER = 65536 / SUMS_RUNS + 1;
+  const float* from = p.partial + (which == 0 ? 0ll : (long long)p.grid * p.D) + col;
+  if (GATES == 0 || which == 0 || (GATES == 2 && which == 1)) {
+    float s = 0.f;
+    if (GATES == 2 && which == 1) {
+      if (there) s = sum_run(from, p.grid, run, PER, p.D, [&](int i) { return value(p.gate + (i * p.gate_per >> 16) * p.ldg); });
+    } else {
+      if (there) s = sum_run(from, p.grid, run, PER, p.D, one);
+    }
     sums[run][lane] = s;
     __syncthreads();
     if (run > 0 || !there) return;
-#pragma unroll
+#pragma unroll 12
     for (int i = 1; i < SUMS_RUNS; ++i) s += sums[i][lane];
-    (which == 0 ? p.grad_weight : p.grad_post)[col] = s;
+    if (which == 0) {
+      p.grad_weight[col] = s;
+    } else {
+      const bool one_gate = GATES == 0 && p.gate && p.ctas_per_gate > 1;
+      if (p.post) p.grad_post[col] = one_gate ? s * value(p.gate) : s;
+      if (one_gate) p.grad_gate[col] = p.post ? s * value(p.post) : s;
+    }
     return;
   }
-  const int runs = sums_runs(p.gates), at = run / runs, part = run - at * runs;
-  const int g = (which - 2) * (SUMS_RUNS / runs) + at, n = p.ctas_per_gate;
-  const bool mine = there && at < SUMS_RUNS / runs && g < p.gates;
-  float s = mine ? sum_run(p.partial + ((long long)2 * p.grid + (long long)g * n) * p.D + col, n, part, runs, p.D) : 0.f;
-  sums[run][lane] = s;
-  __syncthreads();
-  if (part > 0 || !mine) return;
-#pragma unroll
-  for (int i = 1; i < SUMS_RUNS; ++i) s += i < runs ? sums[run + i < SUMS_RUNS ? run + i : 0][lane] : 0.f;
-  p.grad_gate[(long long)g * p.D + col] = s;
+  if constexpr (GATES > 0) {
+    const int runs = p.sums_runs, at = run * p.sums_per >> 16, part = run - at * runs;
+    const int g = (GATES == 2 ? (which - 2) * SUMS_RUNS : 0) + at, n = p.ctas_per_gate;
+    const bool mine = there && g < p.gates;
+    float s = mine ? sum_run(from + (long long)g * n * p.D, n, part, p.sums_per, p.D, one) : 0.f;
+    sums[run][lane] = s;
+    __syncthreads();
+    const bool first = part == 0 && mine;
+    if (first) {
+#pragma unroll 12
+      for (int i = 1; i < SUMS_RUNS; ++i) s += i < runs ? sums[run + i < SUMS_RUNS ? run + i : 0][lane] : 0.f;
+      p.grad_gate[(long long)g * p.D + col] = p.post ? s * value(p.post) : s;
+    }
+    if (GATES == 2 || !p.post) return;
+    if (first) s *= value(p.gate + g * p.ldg);
+    __syncthreads();
+    if (first) sums[at][lane] = s;
+    __syncthreads();
+    if (run > 0 || !there) return;
+    for (int i = 1; i < p.gates; ++i) s += sums[i][lane];
+    p.grad_post[col] = s;
+  }
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------
@@ -922,7 +957,10 @@ static cudaError_t backward_rows(const NormBackwardParams& p, cudaStream_t strea
   return launch_behind(norm_backward_kernel<ACT, F32, V>, dim3((unsigned)p.grid, 1, 1), p.threads, p.smem, stream, p);
 }
 template <int ACT, bool F32>
-static cudaError_t backward_type(const NormBackwardParams& p, cudaStream_t stream) {
+static cudaError_t backward_type(NormBackwardParams p, cudaStream_t stream) {
+  p.sums_runs = p.gates < SUMS_RUNS ? SUMS_RUNS / p.gates : 1;
+  p.sums_per = 65536 / p.sums_runs + 1;
+  p.gate_per = 65536 / p.ctas_per_gate + 1;
   cudaError_t e;
   switch (p.vectors) {
     case 1: e = backward_rows<ACT, F32, 1>(p, stream); break;
@@ -930,9 +968,12 @@ static cudaError_t backward_type(const NormBackwardParams& p, cudaStream_t strea
     default: e = backward_rows<ACT, F32, 4>(p, stream); break;
   }
   if (e != cudaSuccess) return e;
-  const int gates = SUMS_RUNS / sums_runs(p.gates);  // of a CTA
-  const int sums = 2 + (p.grad_gate && p.ctas_per_gate > 1 ? (p.gates + gates - 1) / gates : 0);
-  return launch_behind(norm_sums_kernel, dim3((unsigned)((p.D + 31) / 32), (unsigned)sums, 1), SUMS_RUNS * 32, 0, stream, p);
+  const bool shared = p.ctas_per_gate > 1;
+  const int post = p.post || (shared && p.grad_gate) ? 2 : 1, more = (p.gates + SUMS_RUNS - 1) / SUMS_RUNS;
+  const dim3 grid((unsigned)((p.D + 31) / 32), (unsigned)(shared && p.gates > SUMS_RUNS ? 2 + more : post), 1);
+  if (!shared || p.gates == 1) return launch_behind(norm_sums_kernel<ACT, 0>, grid, SUMS_RUNS * 32, 0, stream, p);
+  if (p.gates <= SUMS_RUNS) return launch_behind(norm_sums_kernel<ACT, 1>, grid, SUMS_RUNS * 32, 0, stream, p);
+  return launch_behind(norm_sums_kernel<ACT, 2>, grid, SUMS_RUNS * 32, 0, stream, p);
 }
 // The shape of the gradient's launch: threads and vectors of a row, CTAs (512 threads to an SM), and stages for the rows ahead.
 void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gate, int sms, int max_smem, NormBackwardParams* p) {
