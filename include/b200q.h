@@ -324,10 +324,11 @@ typedef struct b200q_igemm_plan {
                       3: mma.sync, B straight from memory (M <= 16) */
   int32_t rows;    /* kernel 2: M rounded up to 16 (output only) */
   int32_t width;   /* kernel 1: product columns of a tile, 256 or 128 (gated: half as many outputs); kernel 2: output columns of
-                      a cluster, a multiple of 8 for each of its CTAs, 16 to 256 (gated: 128) */
+                      a cluster, the others being of 8 less, a multiple of 8 up to 256 (gated: 128) */
   int32_t cluster; /* kernel 2: CTAs that share the K of their columns, 1 .. 8 */
   int32_t stages;  /* kernel 2: ring slots of 128 bytes of K, 1 .. 16 */
-  int32_t ctas;    /* kernel 1: CTAs, even; kernel 3: CTAs; kernel 2: output only */
+  int32_t ctas;    /* kernel 1: CTAs, even; kernel 3: CTAs; kernel 2: clusters * cluster; where they are
+                      not as many as columns of that width make, the fewest there can be are taken */
 } b200q_igemm_plan_t;
 int b200q_per_token_cast_int(const void* x, int ldx, void* out, int ldo, float* out_sf, int tokens, int hidden,
                              int act_dtype, void* stream);

@@ -130,10 +130,12 @@ def test_every_plan_gives_the_same_bits(M, N, K, gated):
     first = None
     edits = [dict(kernel=1, width=w, ctas=c) for w, c in ((256, 2), (256, 6), (128, 4), (128, 148))]
     if M <= 256:
-        edits += [dict(kernel=2, width=w * c, cluster=c, stages=s)
-                  for w, c, s in ((16, 1, 1), (48, 1, 3), (24, 1, 2), (56, 1, 2), (120, 1, 2), (80, 1, 3), (128, 1, 2), (16, 2, 4), (64, 2, 1), (16, 3, 2), (32, 4, 3), (8, 2, 2), (24, 2, 2), (56, 2, 1), (24, 4, 2), (8, 8, 1),
-                                  (16, 5, 5), (16, 7, 2), (16, 8, 4), (16, 1, 16))
-                  if c <= -(-K // 128) and (M <= 64 or c < 5 and s < 16) and (gated or w * c >= 16)]  # (what shared memory holds)
+        edits += [dict(kernel=2, width=w, cluster=c, stages=s)
+                  for w, c, s in ((8, 1, 4), (16, 1, 1), (16, 1, 16), (24, 1, 2), (40, 1, 2), (48, 1, 3), (56, 1, 2), (80, 1, 3), (120, 1, 2),
+                                  (128, 1, 2), (8, 2, 2), (16, 2, 2), (24, 2, 2), (32, 2, 4), (56, 2, 3), (112, 2, 1), (128, 2, 1),
+                                  (40, 3, 2), (48, 3, 2), (16, 4, 2), (72, 4, 2), (96, 4, 2), (128, 4, 3), (80, 5, 5), (112, 7, 2), (64, 8, 1),
+                                  (88, 8, 2), (128, 8, 4))
+                  if c <= -(-K // 128) and (M <= 64 or c < 5 and s < 16)]  # (what shared memory holds)
     if M <= 16:
         edits += [dict(kernel=3, ctas=c) for c in (1, 3, 300)]
     for edit in edits:
@@ -153,8 +155,8 @@ def test_plans_that_cannot_run_are_refused():
         assert _planned(a, b, a_sf, b_sf, out, False, **edit) == _lib.ST_OK
     for kernel, edit in ((1, dict(kernel=0)), (1, dict(kernel=4)), (1, dict(width=64)), (1, dict(ctas=3)), (1, dict(ctas=0)),
                          (1, dict(ctas=4096)), (2, dict(cluster=9)),
-                         (2, dict(cluster=5)), (2, dict(cluster=0)), (2, dict(stages=0)), (2, dict(stages=17)), (2, dict(width=72)), (2, dict(cluster=1, width=60)),
-                         (2, dict(width=40)), (2, dict(width=512)), (3, dict(ctas=0))):
+                         (2, dict(cluster=5)), (2, dict(cluster=0)), (2, dict(stages=0)), (2, dict(stages=17)), (2, dict(width=60)), (2, dict(cluster=1, width=4)),
+                         (2, dict(width=0)), (2, dict(width=264)), (3, dict(ctas=0))):
         assert _planned(a, b, a_sf, b_sf, out, False, **{**good[kernel], **edit}) == _lib.ST_UNSUPPORTED, edit
     a, b, a_sf, b_sf = _operands(17, 256, 512)
     out = torch.empty(17, 256, dtype=torch.float16, device="cuda")

@@ -30,8 +30,9 @@ def test_plans():
                         continue
                     assert p["kernel"] == 2 and m <= 256 and p["rows"] == -(-m // 16) * 16 and 2 <= p["stages"] <= 16
                     assert p["cluster"] in (1, 2, 4, 8) and p["cluster"] <= -(-k // 128)
-                    assert p["width"] % (8 * p["cluster"]) == 0 and 16 <= p["width"] <= (128 if gated else 256)
-                    assert p["ctas"] == -(-n // p["width"]) * p["cluster"]
+                    shares = p["ctas"] // p["cluster"]
+                    assert p["ctas"] == shares * p["cluster"] and 1 <= shares <= n // 16
+                    assert p["width"] == -(-(n // 8) // shares) * 8 and 16 <= p["width"] <= (128 if gated else 256)
     for m, n, k in ((1, 24, 128), (1, 128, 24), (1, 16, 131072)):
         with pytest.raises(_lib.B200QError) as e:
             ops.int8_plan(m, n, k)

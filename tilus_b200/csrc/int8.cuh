@@ -20,7 +20,7 @@ struct Int8Params {
   int use_clamp;               // gated: clamp the gate from above and the other factor on both sides
   float clamp;
   int tiles, m_tiles, n_tiles, m_group;  // pair kernel: output tiles and their raster groups
-  int rows, width;             // stream kernel: rows of A rounded up to 16, output columns of a CTA (or of a cluster)
+  int rows, width, wide;       // stream kernel: rows of A rounded up to 16; output columns of the first `wide` CTAs (or clusters)
   int cluster, stages, smem;   // CTAs that share K, ring slots, dynamic shared memory
   int early;                   // stream and row kernels: the kernel before this one does not write B
 };
@@ -39,10 +39,12 @@ EncodeTiledFn encode_tiled_fn();
 
 // int8_kernel.cu
 int int8_pair_smem_bytes(int cols);
-int int8_stream_smem_bytes(int M, int b_rows, int cluster, int stages);
+int int8_stream_smem_bytes(int M, bool gated, int width, int cluster, int stages);
 cudaError_t int8_pair_launch(const Int8Params& p, bool gated, int cols, const CUtensorMap& ta, const CUtensorMap& tb,
                              const CUtensorMap& tc, int grid, cudaStream_t stream);
+int int8_stream_clusters(int s, const DeviceInfo& di);
 cudaError_t int8_row_launch(const Int8Params& p, bool gated, int grid, cudaStream_t stream);
-cudaError_t int8_stream_launch(const Int8Params& p, bool gated, const CUtensorMap& ta, const CUtensorMap& tb, cudaStream_t stream);
+cudaError_t int8_stream_launch(const Int8Params& p, bool gated, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb_less,
+                               cudaStream_t stream);
 
 }  // namespace b200q

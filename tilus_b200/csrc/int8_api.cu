@@ -26,18 +26,21 @@ static int pair_tiles(int M, int N, bool gated, int cols) {
   const int per = gated ? cols / 2 : cols;
   return (int)(((long long)M + 255) / 256 * ((N + per - 1) / per));
 }
-// Output columns of a stream kernel's tile with `s` CTAs to a cluster: an equal share of N for all SMs in as few rounds as the
-// tensor core's 256 columns allow, in units of 8 for each CTA of a cluster.
-static int stream_unit(int s) { return 8 * s; }
-static int stream_width(int N, bool gated, int s, int sms) {
-  const int unit = stream_unit(s), most = (gated ? 128 : 256) / unit * unit, groups = sms / s;
-  const int rounds = (N + most * groups - 1) / (most * groups);
-  const int share = (N + rounds * groups - 1) / (rounds * groups), width = (share + unit - 1) / unit * unit;
-  return width < 16 ? 16 : width;
+// Shares of the columns in the stream kernel, of which `at_once` run at once: as many as that in as few rounds as the tensor core's
+// 256 columns allow, but of two units of 8 columns at least.  They differ by a unit at most.  Where an SM has one, as few as have the widest width, since
+// each reads A (64 x 12288 x 4096 11.6 us with 140, 12.1 with 148); where it has two, all, since what counts is the wider pair of them
+// (64 x 28672 x 4096 gated 21.8 with 256, 21.4 with 296).
+static const int kUnit = 8;
+static int stream_width(int N, int shares) { return (N / kUnit + shares - 1) / shares * kUnit; }  // of the widest
+static int stream_shares(int N, bool gated, int at_once, int per) {
+  const int units = N / kUnit, most = gated ? 16 : 32;
+  const int rounds = (units + most * at_once - 1) / (most * at_once), all = rounds * at_once;
+  const int shares = all < units / 2 ? all : units / 2;
+  return per == 1 ? (N + stream_width(N, shares) - 1) / stream_width(N, shares) : shares;
 }
-static int stream_stages(int M, int b_rows, int s, int budget) {
+static int stream_stages(int M, bool gated, int width, int s, int budget) {
   int stages = 12;  // (with 16 64 x 1024 x 8192 takes 7.3 us, not 7.0)
-  while (stages > 1 && int8_stream_smem_bytes(M, b_rows, s, stages) > budget) --stages;
+  while (stages > 1 && int8_stream_smem_bytes(M, gated, width, s, stages) > budget) --stages;
   return stages;
 }
 
@@ -60,18 +63,21 @@ static double row_cost(int M, double b_bytes, int rounds, int K) {
 static bool split_sectors(int K) { return K % 32 != 0; }
 
 // A piece of 128 bytes of K takes what the slowest of three takes: reading B, bringing both operands' rows to the SM (121 GB/s a SM, or half of that),
-// and the tensor core's reading them (about as fast, but whole accumulators' rows of A).  A cluster's exchange goes by its size
-// and rows: 64 x 4096 x 14336 takes 20.1 us alone, 14.5 in pairs, 15.3 in fours; 128 rows 20.7, 17.1, 19.4.  Two CTAs to an SM
+// and the tensor core's reading them (about as fast, but whole accumulators' rows of A).  A cluster's exchange goes by the
+// sums that it moves: 64 x 4096 x 14336 takes 20.1 us alone, 14.5 in pairs, 15.3 in fours; 128 rows 20.7, 17.1, 19.4.  Two CTAs to an SM
 // (`per` 2) share it, but one starts and ends under the other: 8 x 28672 gated 22.5 us with one, 20.6 with two.
-static double stream_cost(int M, int b_rows, int ctas, int s, int per, int K, const DeviceInfo& di) {
-  const int kblocks = igemm_kblocks(K);
-  const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, slots = per * di.sm_count, rounds = (ctas + slots - 1) / slots;
-  const int busy = ctas < slots ? ctas : slots;
-  const double tensor = per * accs * (128 + b_rows) * 1.05e-3, in = per * (rows + b_rows) * (split_sectors(K) ? 2.1e-3 : 1.05e-3);
-  const int sms = busy < 0.95 * di.sm_count ? (int)(0.95 * di.sm_count) : busy;  // an SM alone gets no more of the memory's rate
-  const double memory = 128.0 * b_rows * sms / kHbm * (per == 1 ? 1.08 : 1.03);
+static double stream_cost(int M, int N, bool gated, int shares, int s, int per, int K, const DeviceInfo& di) {
+  const int kblocks = igemm_kblocks(K), both = gated ? 2 : 1, b_rows = both * stream_width(N, shares), ctas = shares * s;
+  const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, slots = per * s * int8_stream_clusters(s, di);
+  const int rounds = (ctas + slots - 1) / slots;
+  const double tensor = per * accs * (128 + b_rows) * (per == 1 ? 0.95e-3 : 1.05e-3);
+  const double in = per * (rows + b_rows) * (split_sectors(K) ? 2.1e-3 : 1.05e-3);
+  // all of B's rows at the memory's rate, and those of the SM that has most at its own
+  const double all = (double)both * N * s / rounds, alone = (double)both * kUnit * ((per * (N / kUnit) + shares - 1) / shares);
+  const double most = 0.95 * di.sm_count * alone;
+  const double memory = 128.0 / kHbm * (all > most ? all : most) * (per == 1 ? 1.08 : 1.03);
   const double piece = tensor > in ? (tensor > memory ? tensor : memory) : (in > memory ? in : memory);
-  return (per == 1 ? 2.8 : 2.6) + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.2 + 0.05 * s + 0.012 * s * M * busy / slots : 0.0) +
+  return (per == 1 ? 2.8 : 2.6) + rounds * piece * ((kblocks + s - 1) / s) + (s > 1 ? 0.55 + 0.17 * s + 5e-4 * M * b_rows * (s - 1) / s : 0.0) +
          0.004 * per * M;
 }
 
@@ -104,20 +110,20 @@ static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) 
   }
   if (M > kStreamRows) return;
   for (int s = 1; s <= 8 && 4 * (s - 1) <= kblocks; s *= 2)
-    for (int per = s == 1 && kblocks >= 16 ? 2 : 1; per >= 1; --per) {
-      const int width = stream_width(N, gated, s, per * di.sm_count), b_rows = gated ? 2 * width : width;
-      const int ctas = (N + width - 1) / width * s;
-      const double cost = stream_cost(M, b_rows, ctas, s, per, K, di);
+    for (int per = s == 1 && kblocks >= 10 ? 2 : 1; per >= 1; --per) {
+      const int shares = stream_shares(N, gated, per * int8_stream_clusters(s, di), per), width = stream_width(N, shares);
+      if (per == 2 && (M > 128 ? 2 : 1) * (((gated ? 2 : 1) * width + 15) / 16 * 16) > 256) continue;  // (both CTAs' tensor memory)
+      const double cost = stream_cost(M, N, gated, shares, s, per, K, di);
       if (cost >= best) continue;
       // Half an SM's shared memory for one of two CTAs, or where that is depth enough for the length of K: a CTA of the stream's next
       // launch has room next to it then.  (us, K 1024 / 2048 / 4096, half an SM's stages / ten of a whole one's: 24 x 9472, 8 stages, 4.4
       // 7.6 10.7 / 5.0 7.7 10.1; 100 x 9472, 4 stages, 5.4 8.6 12.8 / 5.6 8.0 10.5; 24 x 4736, 12 stages, 3.8 5.2 8.4 / 4.2 5.8 9.0.)
       // A cluster has whole SMs in any case.
-      int stages = stream_stages(M, b_rows, s, s > 1 ? di.max_smem : 113 * 1024);
-      if (s == 1 && per == 1 && stages < 12 && (stages < 3 || 3 * kblocks > 8 * stages)) stages = stream_stages(M, b_rows, s, di.max_smem);
+      int stages = stream_stages(M, gated, width, s, s > 1 ? di.max_smem : 113 * 1024);
+      if (s == 1 && per == 1 && stages < 12 && (stages < 3 || 3 * kblocks > 8 * stages)) stages = stream_stages(M, gated, width, s, di.max_smem);
       if (stages < (per == 1 ? 2 : 3)) continue;
       best = cost;
-      *pl = {2, (M + 15) / 16 * 16, width, s, stages, ctas};
+      *pl = {2, (M + 15) / 16 * 16, width, s, stages, shares * s};
     }
   if (M <= 16) {
     const int items = N / (gated ? 8 : 16);
@@ -165,7 +171,7 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
   p.use_clamp = use_clamp ? 1 : 0;
   p.clamp = clamp;
   const long long b_rows = gated ? 2ll * N : N;
-  CUtensorMap ta, tb, tc;
+  CUtensorMap ta, tb, tb_less, tc;
   cudaError_t e;
   if (pl.kernel == 3) {
     e = int8_row_launch(p, gated, pl.ctas, stream);
@@ -192,13 +198,16 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
   } else {
     st = encode_rows(enc, &ta, a, K, M, lda, pl.rows);
     if (st == ST_OK) st = encode_rows(enc, &tb, b, K, b_rows, ldb, pl.width);
-    if (st != ST_OK) return st;
+    p.tiles = pl.ctas / pl.cluster;
     p.rows = pl.rows; p.width = pl.width; p.cluster = pl.cluster; p.stages = pl.stages;
+    p.wide = p.tiles - (int)((long long)pl.width / kUnit * p.tiles - N / kUnit);
+    if (p.wide == p.tiles) tb_less = tb;
+    else if (st == ST_OK) st = encode_rows(enc, &tb_less, b, K, b_rows, ldb, pl.width - kUnit);
+    if (st != ST_OK) return st;
     // A cluster's CTAs have an SM each to themselves.  Next to one another, two clusters (of one launch or of two streams) could each
     // hold the tensor memory that the other's second CTA waits for.
-    p.smem = pl.cluster > 1 ? device_info().max_smem : int8_stream_smem_bytes(M, gated ? 2 * pl.width : pl.width, 1, pl.stages);
-    p.tiles = pl.ctas / pl.cluster;
-    e = int8_stream_launch(p, gated, ta, tb, stream);
+    p.smem = pl.cluster > 1 ? device_info().max_smem : int8_stream_smem_bytes(M, gated, pl.width, 1, pl.stages);
+    e = int8_stream_launch(p, gated, ta, tb, tb_less, stream);
   }
   return e == cudaSuccess ? ST_OK : cuda_failed((int)e);
 }
@@ -215,10 +224,14 @@ static bool igemm_plan_ok(int M, int N, int K, bool gated, b200q_igemm_plan_t* p
   if (pl->kernel != 2 || M > kStreamRows) return false;
   pl->rows = (M + 15) / 16 * 16;
   if (pl->cluster < 1 || pl->cluster > 8 || pl->cluster > igemm_kblocks(K)) return false;
-  if (pl->width < 16 || pl->width > (gated ? 128 : 256) || pl->width % stream_unit(pl->cluster) != 0) return false;
-  pl->ctas = (N + pl->width - 1) / pl->width * pl->cluster;
+  if (pl->width < kUnit || pl->width > (gated ? 128 : 256) || pl->width % kUnit != 0) return false;
+  // (shares as the CTAs say, where these are of that width; else as few as there can be)
+  int shares = pl->ctas > 0 && pl->ctas % pl->cluster == 0 ? pl->ctas / pl->cluster : 0;
+  if (shares < 1 || shares > N / kUnit || stream_width(N, shares) != pl->width) shares = (N + pl->width - 1) / pl->width;
+  pl->width = stream_width(N, shares);
+  pl->ctas = shares * pl->cluster;
   return pl->stages >= 1 && pl->stages <= 16 &&
-         int8_stream_smem_bytes(M, gated ? 2 * pl->width : pl->width, pl->cluster, pl->stages) <= di.max_smem;
+         int8_stream_smem_bytes(M, gated, pl->width, pl->cluster, pl->stages) <= di.max_smem;
 }
 
 // ---- row-wise kernels -------------------------------------------------------------------------------------

@@ -350,10 +350,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
 }
 
 // ---- stream kernel ----------------------------------------------------------------------------------------
-// A CTA: all rows of A (lanes of tensor memory; 128, or two accumulators of 128) against `width` output columns, which are as many
-// rows of B, or gated twice as many (gates, then partners), over its share of K.  The width is what spreads B evenly over the SMs, so K
-// is split only where reading A again in each CTA would take longer than B.  Then the CTAs of a cluster own an equal part of the
-// columns each: the others store their sums of these into its shared memory, and it adds them to its own.
+// A CTA: all rows of A (lanes of tensor memory; 128, or two accumulators of 128) against a share of the output columns, which are as many
+// rows of B, or gated twice as many (gates, then partners), over its part of K.  Shares differ by eight columns at most, which is what
+// spreads B evenly over the SMs, so K is split only where reading A again in each CTA would take longer than B.  Then the CTAs of a
+// cluster own a part of the columns each: the others store their sums of these into its shared memory, and it adds them to its own.
 constexpr int S_THREADS = 256;
 // Warps that take turns with a stage's copies: what a thread does for one (a wait, a count, two or three copies) takes it about as long
 // as the tensor core takes for the stage.  100 x 11008 x 4224, us with one / four: 11.9 / 11.5; 64 x 28672 gated: 23.1 / 22.9.
@@ -363,8 +363,8 @@ struct StreamBars {
   uint64_t full[S_STAGES_MAX], empty[S_STAGES_MAX], done;
   uint32_t tmem_base;
   int abort_flag;
-  float b_sf[256];           // the tile's columns: gated, the gates' scales and then their partners'
-  unsigned short bias[256];
+  float b_sf[264];           // the share's columns: gated, the gates' scales and then their partners' (read 16 at a time)
+  unsigned short bias[264];
 };
 static __host__ __device__ int stream_ring_bytes(int rows, int b_rows, int stages) {
   // (the tensor core reads whole accumulators' rows of A: behind the last stage too there is memory)
@@ -374,27 +374,32 @@ static __host__ __device__ int stream_ring_bytes(int rows, int b_rows, int stage
 // their 16-byte stores then meet different banks).  They lie behind the ring where they are small, so that nobody has to wait
 // until the receiver's products have read the ring; else in it.
 constexpr int S_INBOX_APART = 16384;
-static __host__ __device__ int stream_inbox_pitch(int b_rows, int cluster) { return b_rows / cluster * 4 + 16; }
-static __host__ __device__ int stream_inbox_bytes(int M, int b_rows, int cluster) {
-  return cluster > 1 ? (cluster - 1) * M * stream_inbox_pitch(b_rows, cluster) + 64 : 0;  // (sums are read 16 at a time)
+// (of shares of `width` columns: the widest part that a CTA owns)
+static __host__ __device__ int stream_inbox_pitch(bool gated, int width, int cluster) {
+  return (width / 8 + cluster - 1) / cluster * 8 * (gated ? 2 : 1) * 4 + 16;
 }
-int int8_stream_smem_bytes(int M, int b_rows, int cluster, int stages) {
-  const int inbox = stream_inbox_bytes(M, b_rows, cluster), ring = stream_ring_bytes((M + 15) / 16 * 16, b_rows, stages);
+static __host__ __device__ int stream_inbox_bytes(int M, bool gated, int width, int cluster) {
+  return cluster > 1 ? (cluster - 1) * M * stream_inbox_pitch(gated, width, cluster) + 64 : 0;  // (sums are read 16 at a time)
+}
+int int8_stream_smem_bytes(int M, bool gated, int width, int cluster, int stages) {
+  const int inbox = stream_inbox_bytes(M, gated, width, cluster);
+  const int ring = stream_ring_bytes((M + 15) / 16 * 16, (gated ? 2 : 1) * width, stages);
   const int data = inbox <= S_INBOX_APART ? ring + inbox : ring > inbox ? ring : inbox;
   return 1024 + data + (int)sizeof(StreamBars);
 }
 
 __device__ __forceinline__ void stream_load_b(const Int8Params& p, const CUtensorMap* tb, bool gated, uint32_t dst, uint32_t bar, int kb,
-                                              int n0) {
+                                              int n0, int width) {
   for (int h = 0; h < (gated ? 2 : 1); ++h)
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst + (uint32_t)(h * p.width) * 128u), "l"(tb), "r"(bar), "r"(kb * 128), "r"(n0 + h * p.N) : "memory");
+        ::"r"(dst + (uint32_t)(h * width) * 128u), "l"(tb), "r"(bar), "r"(kb * 128), "r"(n0 + h * p.N) : "memory");
 }
 
 template <bool GATED>
 __global__ void __launch_bounds__(S_THREADS)
-    int8_stream_kernel(const Int8Params p, const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb) {
+    int8_stream_kernel(const Int8Params p, const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                       const __grid_constant__ CUtensorMap tb_less) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
   const uint32_t bars_s = raw;
@@ -405,16 +410,19 @@ __global__ void __launch_bounds__(S_THREADS)
   volatile int* abort_flag = &bars->abort_flag;
   const int S = p.cluster;
   const int rank = S > 1 ? (int)cluster_rank() : 0;
-  const int n0 = (S > 1 ? blockIdx.x / S : blockIdx.x) * p.width;
+  // the first `wide` shares are of p.width columns, the others of eight less
+  const int share = S > 1 ? blockIdx.x / S : blockIdx.x, width = share < p.wide ? p.width : p.width - 8;
+  const int n0 = share * (p.width - 8) + 8 * min(share, p.wide);
+  const CUtensorMap* map_b = share < p.wide ? &tb : &tb_less;
   const int kb0 = (int)((long long)p.kblocks * rank / S), kb1 = (int)((long long)p.kblocks * (rank + 1) / S);
-  const int b_rows = GATED ? 2 * p.width : p.width;
+  const int b_rows = GATED ? 2 * width : width;
   const int mma_n = (b_rows + 15) / 16 * 16;  // (what is past B's rows of a stage is rows of A: columns that nobody reads)
   const uint32_t b_bytes = (uint32_t)b_rows * 128u, stage_bytes = b_bytes + (uint32_t)p.rows * 128u;
   const int accs = p.rows > 128 ? 2 : 1;
   uint32_t cols = 32;  // of tensor memory: a power of two
   while (cols < (uint32_t)(accs * mma_n)) cols *= 2;
-  const int pitch = stream_inbox_pitch(b_rows, S);
-  const bool apart = stream_inbox_bytes(p.M, b_rows, S) <= S_INBOX_APART;
+  const int pitch = stream_inbox_pitch(GATED, p.width, S);
+  const bool apart = stream_inbox_bytes(p.M, GATED, p.width, S) <= S_INBOX_APART;
   const uint32_t inbox = apart ? ring + (uint32_t)stream_ring_bytes(p.rows, b_rows, p.stages) : ring;
 
   if (tid <= p.stages) {
@@ -437,7 +445,7 @@ __global__ void __launch_bounds__(S_THREADS)
       if (p.early)  // rows of B, which the kernel before this one does not write: the first of them come under its end
         for (int i = warp; i < p.stages && kb0 + i < kb1; i += S_COPIERS) {
           expect_bytes(BAR(full, i), stage_bytes);
-          stream_load_b(p, &tb, GATED, ring + (uint32_t)i * stage_bytes, BAR(full, i), kb0 + i, n0);
+          stream_load_b(p, map_b, GATED, ring + (uint32_t)i * stage_bytes, BAR(full, i), kb0 + i, n0, width);
         }
       asm volatile("prefetch.tensormap [%0];" ::"l"(&ta) : "memory");
     }
@@ -452,7 +460,7 @@ __global__ void __launch_bounds__(S_THREADS)
         const uint32_t bar = BAR(full, s), dst = ring + (uint32_t)s * stage_bytes;
         if (!p.early || lap > 0) {
           expect_bytes(bar, stage_bytes);
-          stream_load_b(p, &tb, GATED, dst, bar, kb, n0);
+          stream_load_b(p, map_b, GATED, dst, bar, kb, n0, width);
         }
         asm volatile(
             "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -503,9 +511,8 @@ __global__ void __launch_bounds__(S_THREADS)
   } else {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int i = tid - 32 * (S_COPIERS + 1); i < b_rows; i += S_THREADS - 32 * (S_COPIERS + 1)) {
-      const int n = n0 + (GATED ? i % p.width : i);
-      bars->b_sf[i] = n < p.N ? p.b_sf[GATED && i >= p.width ? n + p.N : n] : 0.f;
-      if (!GATED && p.bias) bars->bias[i] = n < p.N ? p.bias[n] : (unsigned short)0;
+      bars->b_sf[i] = p.b_sf[GATED && i >= width ? n0 + p.N + i - width : n0 + i];
+      if (!GATED && p.bias) bars->bias[i] = p.bias[n0 + i];
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -518,7 +525,8 @@ __global__ void __launch_bounds__(S_THREADS)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const int row = (warp & 3) * 32 + lane, turn = warp >> 2;
   const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  const int own = p.width / S;  // columns that a CTA of the cluster writes
+  // columns that a CTA of the cluster writes, in units of eight
+  const int units = width / 8, own0 = units * rank / S * 8, own = units * (rank + 1) / S * 8 - own0;
   if (S > 1) {
     if (!apart) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA's ring may be written
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -531,7 +539,8 @@ __global__ void __launch_bounds__(S_THREADS)
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i]));  // no use of v moves above the wait
-        const int seg = GATED && j >= p.width ? 1 : 0, c = (j - seg * p.width) / own, at = seg * own + j - seg * p.width - c * own;
+        const int seg = GATED && j >= width ? 1 : 0, unit = j / 8 - seg * units, c = ((unit + 1) * S - 1) / units;
+        const int first = units * c / S, at = 8 * (seg * (units * (c + 1) / S - first) + unit - first);
         if (c != rank && t < p.M) {
           const int slot = rank < c ? rank : rank - 1;  // among the senders to c
           const uint32_t to = map_to(inbox + (uint32_t)((slot * p.M + t) * pitch + at * 4), (uint32_t)c);
@@ -552,15 +561,14 @@ __global__ void __launch_bounds__(S_THREADS)
     const int t = m * 128 + row;
     const float sa = t < p.M ? p.a_sf[t] : 0.f;
     for (int j = 16 * turn; j < own; j += 32) {
-      const int i0 = rank * own + j, n = n0 + i0;  // 16 columns, or the last 8 of the CTA's or of N
-      if (n >= p.N) break;
+      const int i0 = own0 + j, n = n0 + i0;  // 16 columns, or the last 8 of the CTA's
       const bool full = j + 8 < own;
       uint32_t v[16] = {}, u[16] = {};
       tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + i0), v);
       if (full) tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + i0 + 8), v + 8);
       if constexpr (GATED) {
-        tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + p.width + i0), u);
-        if (full) tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + p.width + i0 + 8), u + 8);
+        tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + width + i0), u);
+        if (full) tmem_ld_8_async(lane_addr + (uint32_t)(m * mma_n + width + i0 + 8), u + 8);
       }
       tmem_ld_wait(v);
       if (GATED)
@@ -585,7 +593,7 @@ __global__ void __launch_bounds__(S_THREADS)
       if constexpr (GATED) {
         float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = scaled(u[i], sa, bars->b_sf[p.width + i0 + i]);
+        for (int i = 0; i < 16; ++i) x[i] = scaled(u[i], sa, bars->b_sf[width + i0 + i]);
         gate_all(f, x, p.use_clamp, p.clamp);
       } else if (p.bias) {
         add_bias(p.act, f, bars->bias + i0);
@@ -594,7 +602,7 @@ __global__ void __launch_bounds__(S_THREADS)
       if (t < p.M && *abort_flag == 0) {
         uint4* to = reinterpret_cast<uint4*>(p.c + (size_t)t * p.ldc + n);
         to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        if (full && n + 8 < p.N) to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        if (full) to[1] = make_uint4(o[4], o[5], o[6], o[7]);
       }
       __syncwarp();
     }
@@ -738,11 +746,12 @@ static cudaError_t pair_launch(const Int8Params& p, const CUtensorMap& ta, const
   return launch_behind(int8_pair_kernel<GATED, COLS>, grid, P_THREADS, 1, int8_pair_smem_bytes(COLS), stream, p, ta, tb, tc);
 }
 template <bool GATED>
-static cudaError_t stream_launch(const Int8Params& p, const CUtensorMap& ta, const CUtensorMap& tb, cudaStream_t stream) {
+static cudaError_t stream_launch(const Int8Params& p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb_less,
+                                 cudaStream_t stream) {
   static std::atomic<bool> allowed[16];
   const cudaError_t e = allow_smem(int8_stream_kernel<GATED>, allowed);
   if (e != cudaSuccess) return e;
-  return launch_behind(int8_stream_kernel<GATED>, p.tiles * p.cluster, S_THREADS, p.cluster, p.smem, stream, p, ta, tb);
+  return launch_behind(int8_stream_kernel<GATED>, p.tiles * p.cluster, S_THREADS, p.cluster, p.smem, stream, p, ta, tb, tb_less);
 }
 
 cudaError_t int8_pair_launch(const Int8Params& p, bool gated, int cols, const CUtensorMap& ta, const CUtensorMap& tb,
@@ -750,8 +759,37 @@ cudaError_t int8_pair_launch(const Int8Params& p, bool gated, int cols, const CU
   if (cols == 256) return gated ? pair_launch<true, 256>(p, ta, tb, tc, grid, stream) : pair_launch<false, 256>(p, ta, tb, tc, grid, stream);
   return gated ? pair_launch<true, 128>(p, ta, tb, tc, grid, stream) : pair_launch<false, 128>(p, ta, tb, tc, grid, stream);
 }
-cudaError_t int8_stream_launch(const Int8Params& p, bool gated, const CUtensorMap& ta, const CUtensorMap& tb, cudaStream_t stream) {
-  return gated ? stream_launch<true>(p, ta, tb, stream) : stream_launch<false>(p, ta, tb, stream);
+cudaError_t int8_stream_launch(const Int8Params& p, bool gated, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb_less,
+                               cudaStream_t stream) {
+  return gated ? stream_launch<true>(p, ta, tb, tb_less, stream) : stream_launch<false>(p, ta, tb, tb_less, stream);
+}
+
+// Clusters of s CTAs with an SM each that run at once: fewer than the SMs make, since a cluster stays in a group of SMs.  (Without a
+// GPU an estimate, for plans.)
+int int8_stream_clusters(int s, const DeviceInfo& di) {
+  static std::atomic<int> known[16][9];
+  if (s == 1) return di.sm_count;
+  int dev = -1, n = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 16 && (n = known[dev][s].load(std::memory_order_relaxed)) > 0) return n;
+  static std::atomic<bool> allowed[16];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(di.sm_count / s * s), 1, 1);
+  cfg.blockDim = dim3(S_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)di.max_smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)s;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (dev >= 0 && allow_smem(int8_stream_kernel<false>, allowed) == cudaSuccess &&
+      cudaOccupancyMaxActiveClusters(&n, int8_stream_kernel<false>, &cfg) == cudaSuccess && n > 0) {
+    if (dev < 16) known[dev][s].store(n, std::memory_order_relaxed);
+    return n;
+  }
+  (void)cudaGetLastError();
+  return s == 2 ? di.sm_count / 2 : di.sm_count * 7 / 8 / s;
 }
 
 cudaError_t int8_row_launch(const Int8Params& p, bool gated, int grid, cudaStream_t stream) {
