@@ -335,6 +335,23 @@ def test_weights_cast_on_another_stream_of_a_captured_graph(M):
         assert torch.equal(out, want * sign)
 
 
+def test_products_on_two_streams_at_once():
+    """Clusters, pairs and two CTAs to an SM of two streams next to one another."""
+    shapes = [(64, 1024, 8192, False), (200, 528, 4096, False), (64, 28672, 1024, True), (300, 2048, 1024, False), (9, 4096, 8192, False)]
+    sets = [_operands(m, n, k, seed=i) for i, (m, n, k, _) in enumerate(shapes)]
+    call = lambda o, gated: ops.int8_gate_up(*o) if gated else ops.int8_matmul(*o)
+    wants = [call(o, s[3]) for o, s in zip(sets, shapes)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(40):
+        for k, stream in enumerate(streams):
+            j = (i + 2 * k) % len(shapes)
+            with torch.cuda.stream(stream):
+                got.append((j, call(sets[j], shapes[j][3])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, wants[j]) for j, out in got)
+
+
 def test_other_streams_and_captured_graphs():
     torch.manual_seed(2)
     layer = Int8Linear(torch.bfloat16, 1024, 2048).cuda()

@@ -42,7 +42,7 @@ int int8_pair_smem_bytes(int cols);
 int int8_stream_smem_bytes(int M, bool gated, int width, int cluster, int stages);
 cudaError_t int8_pair_launch(const Int8Params& p, bool gated, int cols, const CUtensorMap& ta, const CUtensorMap& tb,
                              const CUtensorMap& tc, int grid, cudaStream_t stream);
-int int8_stream_clusters(int s, const DeviceInfo& di);
+const int* int8_stream_clusters(const DeviceInfo& di);
 cudaError_t int8_row_launch(const Int8Params& p, bool gated, int grid, cudaStream_t stream);
 cudaError_t int8_stream_launch(const Int8Params& p, bool gated, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb_less,
                                cudaStream_t stream);

@@ -27,9 +27,9 @@ static int pair_tiles(int M, int N, bool gated, int cols) {
   return (int)(((long long)M + 255) / 256 * ((N + per - 1) / per));
 }
 // Shares of the columns in the stream kernel, of which `at_once` run at once: as many as that in as few rounds as the tensor core's
-// 256 columns allow, but of two units of 8 columns at least.  They differ by a unit at most.  Where an SM has one, as few as have the widest width, since
-// each reads A (64 x 12288 x 4096 11.6 us with 140, 12.1 with 148); where it has two, all, since what counts is the wider pair of them
-// (64 x 28672 x 4096 gated 21.8 with 256, 21.4 with 296).
+// 256 columns allow, but of two units of 8 columns at least.  They differ by a unit at most.  Where an SM
+// has one, as few as have the widest width, since each reads A (64 x 12288 x 4096 11.6 us with 140, 12.1 with 148); where it has two,
+// all, since what counts is the wider pair of them (64 x 28672 x 4096 gated 21.8 with 256, 21.4 with 296).
 static const int kUnit = 8;
 static int stream_width(int N, int shares) { return (N / kUnit + shares - 1) / shares * kUnit; }  // of the widest
 static int stream_shares(int N, bool gated, int at_once, int per) {
@@ -62,13 +62,13 @@ static double row_cost(int M, double b_bytes, int rounds, int K) {
 // 1024 x 18944 50 / 53 / 65, 200 x 4736 12.9 / 14.1 / 19.7.)
 static bool split_sectors(int K) { return K % 32 != 0; }
 
-// A piece of 128 bytes of K takes what the slowest of three takes: reading B, bringing both operands' rows to the SM (121 GB/s a SM, or half of that),
-// and the tensor core's reading them (about as fast, but whole accumulators' rows of A).  A cluster's exchange goes by the
+// A piece of 128 bytes of K takes what the slowest of three takes: reading B, bringing both operands' rows to the SM (121 GB/s a SM, or
+// half of that), and the tensor core's reading them (about as fast, but whole accumulators' rows of A).  A cluster's exchange goes by the
 // sums that it moves: 64 x 4096 x 14336 takes 20.1 us alone, 14.5 in pairs, 15.3 in fours; 128 rows 20.7, 17.1, 19.4.  Two CTAs to an SM
 // (`per` 2) share it, but one starts and ends under the other: 8 x 28672 gated 22.5 us with one, 20.6 with two.
-static double stream_cost(int M, int N, bool gated, int shares, int s, int per, int K, const DeviceInfo& di) {
+static double stream_cost(int M, int N, bool gated, int shares, int s, int at_once, int per, int K, const DeviceInfo& di) {
   const int kblocks = igemm_kblocks(K), both = gated ? 2 : 1, b_rows = both * stream_width(N, shares), ctas = shares * s;
-  const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, slots = per * s * int8_stream_clusters(s, di);
+  const int rows = (M + 15) / 16 * 16, accs = (rows + 127) / 128, slots = s * at_once;
   const int rounds = (ctas + slots - 1) / slots;
   const double tensor = per * accs * (128 + b_rows) * (per == 1 ? 0.95e-3 : 1.05e-3);
   const double in = per * (rows + b_rows) * (split_sectors(K) ? 2.1e-3 : 1.05e-3);
@@ -109,11 +109,12 @@ static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) 
     *pl = {1, 256, cols, 2, cols == 256 ? 6 : 8, 2 * (tiles < di.sm_count / 2 ? tiles : di.sm_count / 2)};
   }
   if (M > kStreamRows) return;
-  for (int s = 1; s <= 8 && 4 * (s - 1) <= kblocks; s *= 2)
+  const int* clusters = int8_stream_clusters(di);
+  for (int s = 1, i = 0; s <= 8 && 4 * (s - 1) <= kblocks; s *= 2, ++i)
     for (int per = s == 1 && kblocks >= 10 ? 2 : 1; per >= 1; --per) {
-      const int shares = stream_shares(N, gated, per * int8_stream_clusters(s, di), per), width = stream_width(N, shares);
+      const int at_once = per * clusters[i], shares = stream_shares(N, gated, at_once, per), width = stream_width(N, shares);
       if (per == 2 && (M > 128 ? 2 : 1) * (((gated ? 2 : 1) * width + 15) / 16 * 16) > 256) continue;  // (both CTAs' tensor memory)
-      const double cost = stream_cost(M, N, gated, shares, s, per, K, di);
+      const double cost = stream_cost(M, N, gated, shares, s, at_once, per, K, di);
       if (cost >= best) continue;
       // Half an SM's shared memory for one of two CTAs, or where that is depth enough for the length of K: a CTA of the stream's next
       // launch has room next to it then.  (us, K 1024 / 2048 / 4096, half an SM's stages / ten of a whole one's: 24 x 9472, 8 stages, 4.4

@@ -26,6 +26,8 @@
 // row-wise kernels they let the kernel behind them start only after their own wait, so that whatever runs then, the kernel
 // before the last has ended; and only once they have their tensor memory, which a CTA behind them, waiting for their end, could
 // otherwise hold.
+#include <mutex>
+
 #include "int8.cuh"
 #include "umma_common.cuh"
 
@@ -499,7 +501,8 @@ __global__ void __launch_bounds__(S_THREADS)
                 "{\n\t.reg .pred p;\n\t"
                 "setp.ne.b32 p, %4, 0;\n\t"
                 "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-                ::"r"(tmem + (uint32_t)(m * mma_n)), "l"(ad + (uint64_t)(m * 1024 + ks * 2)), "l"(bd + (uint64_t)(ks * 2)), "r"(idesc), "r"((kb > kb0 || ks > 0) ? 1u : 0u)
+                ::"r"(tmem + (uint32_t)(m * mma_n)), "l"(ad + (uint64_t)(m * 1024 + ks * 2)), "l"(bd + (uint64_t)(ks * 2)), "r"(idesc),
+                "r"((kb > kb0 || ks > 0) ? 1u : 0u)
                 : "memory");
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(BAR(empty, s)) : "memory");
         if (++s == p.stages) { s = 0; phase ^= 1u; }
@@ -764,32 +767,39 @@ cudaError_t int8_stream_launch(const Int8Params& p, bool gated, const CUtensorMa
   return gated ? stream_launch<true>(p, ta, tb, tb_less, stream) : stream_launch<false>(p, ta, tb, tb_less, stream);
 }
 
-// Clusters of s CTAs with an SM each that run at once: fewer than the SMs make, since a cluster stays in a group of SMs.  (Without a
-// GPU an estimate, for plans.)
-int int8_stream_clusters(int s, const DeviceInfo& di) {
-  static std::atomic<int> known[16][9];
-  if (s == 1) return di.sm_count;
-  int dev = -1, n = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 16 && (n = known[dev][s].load(std::memory_order_relaxed)) > 0) return n;
-  static std::atomic<bool> allowed[16];
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(di.sm_count / s * s), 1, 1);
-  cfg.blockDim = dim3(S_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = (size_t)di.max_smem;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)s;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (dev >= 0 && allow_smem(int8_stream_kernel<false>, allowed) == cudaSuccess &&
-      cudaOccupancyMaxActiveClusters(&n, int8_stream_kernel<false>, &cfg) == cudaSuccess && n > 0) {
-    if (dev < 16) known[dev][s].store(n, std::memory_order_relaxed);
-    return n;
+// Clusters of 1 << i CTAs with an SM each that run at once: fewer than the SMs make, since a cluster stays in a group of SMs.  (Without
+// a GPU estimates, for plans.)
+const int* int8_stream_clusters(const DeviceInfo& di) {
+  static std::atomic<bool> known[16], allowed[16];
+  static int counts[17][4];
+  static std::mutex mutex;
+  int dev = -1;
+  const bool gpu = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 16;
+  const int at = gpu ? dev : 16;
+  if (gpu && known[dev].load(std::memory_order_acquire)) return counts[dev];
+  std::lock_guard<std::mutex> lock(mutex);
+  for (int i = 0, s = 1; i < 4; ++i, s *= 2) {
+    int n = 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(di.sm_count / s * s), 1, 1);
+    cfg.blockDim = dim3(S_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)di.max_smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (s > 1 && (!gpu || allow_smem(int8_stream_kernel<false>, allowed) != cudaSuccess ||
+                  cudaOccupancyMaxActiveClusters(&n, int8_stream_kernel<false>, &cfg) != cudaSuccess || n < 1)) {
+      (void)cudaGetLastError();
+      n = s == 2 ? di.sm_count / 2 : di.sm_count * 7 / 8 / s;
+    }
+    counts[at][i] = s > 1 ? n : di.sm_count;
   }
-  (void)cudaGetLastError();
-  return s == 2 ? di.sm_count / 2 : di.sm_count * 7 / 8 / s;
+  if (gpu) known[dev].store(true, std::memory_order_release);
+  return counts[at];
 }
 
 cudaError_t int8_row_launch(const Int8Params& p, bool gated, int grid, cudaStream_t stream) {

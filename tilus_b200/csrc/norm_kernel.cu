@@ -516,7 +516,9 @@ __global__ void __launch_bounds__(256, 2) norm_rows_kernel(const NormParams p) {
 //
 // A CTA takes a run of rows of one gate and keeps its share of the sums over rows in registers; a second kernel adds the CTAs' shares
 // in a fixed order, so that a call gives the same bits each time.  Rows are copied to shared memory ahead of their turn
-// by the copy engine: with a row at a time in registers and three reductions 8192 x 5120 took 386 us, of a floor of 117.
+// by the copy engine.  8192 x 5120 with a 32-bit residual and 8 gates takes 148 us (5.1 TB/s; with a row at a time in registers and three
+// reductions 386), 511 x 4096 with a gate 13.9: what bounds it is the latency of a row's reduction between its copies and its outputs, at
+// as many rows on an SM as registers allow.
 // The sums of eight values over the CTA's threads, in every thread.  Halving exchanges: after the steps over 16, 8 and 4 lanes a lane
 // holds one value, lane >> 2; so a warp's part takes 9 shuffles instead of 40.  `slots`: 8 words a warp, of two sets in turn.
 __device__ __forceinline__ void sums8(float (&v)[8], float* slots) {
@@ -881,8 +883,8 @@ static cudaError_t launch_behind(Kernel kern, dim3 grid, int threads, int smem, 
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// Threads of a row and vectors of a thread: a warp for up to 512 channels (2048 where rows are many), else a CTA.  Where rows are many, 256 threads with up to
-// eight vectors, so that the steps of a reduction are shared by many channels; where they are few, as many as the row has.
+// Threads of a row and vectors of a thread: a warp for up to 512 channels (2048 where rows are many), else a CTA.  Where rows are many,
+// 256 threads with up to eight vectors, so that the steps of a reduction are shared by many channels; where they are few, as many as the row has.
 struct RowShape { int warp_rows, threads, vectors, ctas; };
 static RowShape row_shape(int T, int D) {
   const int nvec = D / 8;
