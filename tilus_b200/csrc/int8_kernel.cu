@@ -17,9 +17,9 @@
 //           epilogue runs under the next one's products.  For many rows: bound by the tensor cores.
 //   stream  up to 256 rows, all of them against an equal share of the columns in each CTA, so that B is read once: bound by that.
 //   row     up to 16 rows where the product is small: no pipeline to fill, mma.sync from registers.  Bound by the latency of its loads.
-// On a B200, between launches of a graph: pair, 4096 x 8192 x 8192, 162 us (3.40 POP/s, the tensor pipe busy 88 % of the time); 4096 x 28672
-// x 8192 gated 562 to 641 us as the power limit has it (3.0 to 3.4 POP/s); stream, 8 x 28672 x 4096 gated 20.6 us (5.7 TB/s), 1 x 16384 x
-// 8192 27 us, 64 x 28672 x 4096 gated 23 us; row, 1 x 4096 x 4096 4.1 us.
+// On a B200, in a graph of such calls: pair, 4096 x 8192 x 8192, 162 us (3.40 POP/s, the tensor pipe busy 88 % of the time); 4096 x 28672
+// x 8192 gated 558 to 642 us as the power limit has it (3.0 to 3.4 POP/s); stream, 8 x 28672 x 4096 gated 20.5 us (5.7 TB/s), 1 x 16384 x
+// 8192 23.6 us (5.7 TB/s), 64 x 28672 x 4096 gated 21.4 us; row, 1 x 4096 x 4096 3.6 us.
 //
 // All are launched with programmatic stream serialization: they set up under the end of the kernel before them.  All they read
 // before that kernel has ended is, in the stream and row kernels and where the caller says that it may (`early`), rows of B.  Like the
@@ -358,7 +358,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
 // cluster own a part of the columns each: the others store their sums of these into its shared memory, and it adds them to its own.
 constexpr int S_THREADS = 256;
 // Warps that take turns with a stage's copies: what a thread does for one (a wait, a count, two or three copies) takes it about as long
-// as the tensor core takes for the stage.  100 x 11008 x 4224, us with one / four: 11.9 / 11.5; 64 x 28672 gated: 23.1 / 22.9.
+// as the tensor core takes for the stage.  100 x 11008 x 4224, us with one / four: 11.9 / 11.5.
 constexpr int S_COPIERS = 4;
 constexpr int S_STAGES_MAX = 16;
 struct StreamBars {
