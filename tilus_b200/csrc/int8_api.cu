@@ -49,12 +49,12 @@ static int stream_stages(int M, bool gated, int width, int s, int budget) {
 constexpr double kHbm = 6465.5e3;  // bytes a us
 
 // Reading B at five sixths of the memory's rate up to eight rows of A (with twice as many, whose loads are as many as B's, at three
-// fifths), but no less than the latency of each round of a CTA and of each 4096 bytes of K in it.
+// fifths), but no less than the latency of each round of a CTA, which goes by its length of K.
 static double row_cost(int M, double b_bytes, int rounds, int K) {
   const bool few = M <= 8;
-  const int more = (K - 1) / 4096;
+  const double steps = K / 4096.0;
   const double memory = 1.6 + b_bytes / kHbm * (few ? 1.2 : 1.62);
-  const double latency = 0.4 + rounds * (few ? 1.5 + 1.7 * more : 2.0 + 2.8 * more);
+  const double latency = 0.4 + rounds * (few ? 1.4 + 1.4 * steps : 1.9 + 2.4 * steps);
   return memory > latency ? memory : latency;
 }
 
