@@ -94,7 +94,7 @@ static double pair_cost(int tiles, bool gated, int cols, int K, double b_bytes, 
   return start + (all > memory ? all : memory);
 }
 
-static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) {
+static void make_igemm_plan(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) {
   const DeviceInfo di = device_info();
   const int kblocks = igemm_kblocks(K);
   *pl = b200q_igemm_plan_t();
@@ -131,6 +131,20 @@ static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) 
     const double cost = row_cost(M, (double)(gated ? 2 : 1) * N * K, (items + 2 * di.sm_count - 1) / (2 * di.sm_count), K);
     if (cost < best) *pl = {3, M, gated ? 8 : 16, 1, 1, items < 2 * di.sm_count ? items : 2 * di.sm_count};
   }
+}
+
+// A thread's latest plans: a model's layers come again with each token, and to weigh the kernels takes a tenth of a small call (0.3 us).
+static void plan_igemm(int M, int N, int K, bool gated, b200q_igemm_plan_t* pl) {
+  struct Known { int M = 0, N, K, gated, dev; b200q_igemm_plan_t plan; };
+  static thread_local Known known[16];
+  int dev = -1;
+  (void)cudaGetDevice(&dev);
+  Known& k = known[((unsigned)N / 16 * 7 + (unsigned)K / 16 * 3 + (unsigned)M + (gated ? 5 : 0)) % 16];
+  if (k.M != M || k.N != N || k.K != K || k.gated != (int)gated || k.dev != dev) {
+    make_igemm_plan(M, N, K, gated, &k.plan);
+    k.M = M; k.N = N; k.K = K; k.gated = gated; k.dev = dev;
+  }
+  *pl = k.plan;
 }
 
 // 2-D map of 8-bit rows, a box of 128 bytes x `rows`
