@@ -150,6 +150,13 @@ def test_gradients_of_several_gates(T, gates, post):
     _check_gradients(_make(T, 264, torch.bfloat16, wide=True, post=post, gates=gates, grads=True), 1.0)
 
 
+@pytest.mark.parametrize("T,gates", [(9, 1), (60, 3), (90, 30), (5, 0)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_gradients_of_gates_of_wide_rows(T, gates, dtype):
+    """Above 4096 channels the sums are taken over pairs of them."""
+    _check_gradients(_make(T, 4168, dtype, post=True, gates=gates, grads=True), 0.5)
+
+
 def test_gradients_without_one_of_the_new_residual():
     s = _make(40, 1000, torch.float16, post=True, gates=1, grads=True)
     s["grad_new"] = None

@@ -788,46 +788,102 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
   }
 }
 
-// The sums of the CTAs' shares: 32 columns a CTA, 24 runs of shares side by side, joined in order.  A thread's loads, which come from L2,
-// are under way together: seven are a CTA to each SM.  (511 x 4096, us for the whole gradient: 8 runs and a loop unrolled ten times,
-// whose rest went one by one, 15.7; 8 runs in tens 14.4, 16 in tens 13.3, 24 in sevens 12.7.)  blockIdx.y: grad_weight, grad_post
-// and up to 24 gates, whose runs are the fewer the more they are; more gates after that.  (Quotients by products: several divisions of a
-// thread's cost 0.3 us.)
+// The sums of the CTAs' shares: 32 columns a CTA (pairs of columns from 4104 on, so that all
+// CTAs run at once: 148 x 8192 with a 32-bit residual 13.5 / 12.9 us), 24 runs of shares side by
+// side, joined in order.  A thread's loads, which come from L2, are under way together: seven are a CTA to each SM.  (511 x 4096, us for
+// the whole gradient: 8 runs and a loop unrolled ten times, whose rest went one by one, 15.7; 8 runs in tens 14.4, 16 in tens 13.3,
+// 24 in sevens 12.7.)  blockIdx.y: grad_weight, grad_post and up to 24 gates, whose runs are the fewer the more they are; more
+// gates after that.  (Quotients by products: several divisions of a thread's cost 0.3 us.)
 constexpr int SUMS_RUNS = 24, SUMS_BATCH = 7;
-// Run `part` of n shares at `from`, `factor(share)` in front of each.  The runs meet at n * part / (runs), taken as a product with `per` =
+template <int C>
+struct Cols {  // a thread's columns
+  float v[C];
+  __device__ __forceinline__ void load(const float* p) {
+    if constexpr (C == 2) {
+      const float2 t = *reinterpret_cast<const float2*>(p);
+      v[0] = t.x; v[1] = t.y;
+    } else {
+      v[0] = *p;
+    }
+  }
+  template <int ACT>
+  __device__ __forceinline__ void load16(const unsigned short* p) {
+    if constexpr (C == 2) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+      if constexpr (ACT == 0) {
+        const float2 t = __half22float2(h2_from_bits(w));
+        v[0] = t.x; v[1] = t.y;
+      } else {
+        v[0] = __uint_as_float(w << 16); v[1] = __uint_as_float(w & 0xffff0000u);
+      }
+    } else {
+      v[0] = ACT == 0 ? __half2float(__ushort_as_half(*p)) : __uint_as_float((uint32_t)*p << 16);
+    }
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    if constexpr (C == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    else *p = v[0];
+  }
+  __device__ __forceinline__ void set(float x) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) v[c] = x;
+  }
+  __device__ __forceinline__ Cols operator*(const Cols& o) const {
+    Cols r;
+#pragma unroll
+    for (int c = 0; c < C; ++c) r.v[c] = v[c] * o.v[c];
+    return r;
+  }
+  __device__ __forceinline__ void operator+=(const Cols& o) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) v[c] += o.v[c];
+  }
+};
+// Run `part` of n shares at `from`, `weigh(share, values)` in between.  The runs meet at n * part / (runs), taken as a product with `per` =
 // 65536 / runs + 1 (up to a few thousand shares the last one ends at n: the product is too large by less than one).
-template <class Factor>
-__device__ __forceinline__ float sum_run(const float* from, int n, int part, int per, long long D, Factor factor) {
-  float s = 0.f;
+template <int C, class Weigh>
+__device__ __forceinline__ Cols<C> sum_run(const float* from, int n, int part, int per, long long D, Weigh weigh) {
+  Cols<C> s;
+  s.set(0.f);
   const int i1 = (int)((unsigned)(n * (part + 1)) * (unsigned)per >> 16);
   for (int i = (int)((unsigned)(n * part) * (unsigned)per >> 16); i < i1; i += SUMS_BATCH) {
-    float x[SUMS_BATCH];
+    Cols<C> x[SUMS_BATCH];
 #pragma unroll
-    for (int j = 0; j < SUMS_BATCH; ++j) x[j] = i + j < i1 ? from[(i + j) * D] * factor(i + j) : 0.f;
+    for (int j = 0; j < SUMS_BATCH; ++j) {
+      x[j].set(0.f);
+      if (i + j < i1) {
+        x[j].load(from + (i + j) * D);
+        weigh(i + j, x[j]);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < SUMS_BATCH; ++j) s += x[j];
   }
   return s;
 }
 // GATES: 0 one gate, none or CTAs that leave nothing for several to be done; else CTAs share several gates, 1 up to 24, 2 more.
-template <int ACT, int GATES>
+template <int ACT, int GATES, int C>
 __global__ void __launch_bounds__(SUMS_RUNS * 32, 2) norm_sums_kernel(const NormBackwardParams p) {
-  __shared__ float sums[SUMS_RUNS][33];
+  __shared__ Cols<C> sums[SUMS_RUNS][33];
   start_behind();
-  const int which = (int)blockIdx.y, lane = threadIdx.x & 31, col = (int)blockIdx.x * 32 + lane, run = threadIdx.x >> 5;
+  const int which = (int)blockIdx.y, lane = threadIdx.x & 31, col = ((int)blockIdx.x * 32 + lane) * C, run = threadIdx.x >> 5;
   const bool there = col < p.D;
   auto value = [&](const unsigned short* from) {
-    return ACT == 0 ? __half2float(__ushort_as_half(from[col])) : __uint_as_float((uint32_t)from[col] << 16);
+    Cols<C> x;
+    x.template load16<ACT>(from + col);
+    return x;
   };
-  const auto one = [](int) { return 1.f; };
+  const auto as_is = [](int, Cols<C>&) {};
   constexpr int PER = 65536 / SUMS_RUNS + 1;
   const float* from = p.partial + (which == 0 ? 0ll : (long long)p.grid * p.D) + col;
   if (GATES == 0 || which == 0 || (GATES == 2 && which == 1)) {
-    float s = 0.f;
+    Cols<C> s;
+    s.set(0.f);
     if (GATES == 2 && which == 1) {
-      if (there) s = sum_run(from, p.grid, run, PER, p.D, [&](int i) { return value(p.gate + (i * p.gate_per >> 16) * p.ldg); });
+      if (there)
+        s = sum_run<C>(from, p.grid, run, PER, p.D, [&](int i, Cols<C>& x) { x = x * value(p.gate + (i * p.gate_per >> 16) * p.ldg); });
     } else {
-      if (there) s = sum_run(from, p.grid, run, PER, p.D, one);
+      if (there) s = sum_run<C>(from, p.grid, run, PER, p.D, as_is);
     }
     sums[run][lane] = s;
     __syncthreads();
@@ -835,11 +891,11 @@ __global__ void __launch_bounds__(SUMS_RUNS * 32, 2) norm_sums_kernel(const Norm
 #pragma unroll 12
     for (int i = 1; i < SUMS_RUNS; ++i) s += sums[i][lane];
     if (which == 0) {
-      p.grad_weight[col] = s;
+      s.store(p.grad_weight + col);
     } else {
       const bool one_gate = GATES == 0 && p.gate && p.ctas_per_gate > 1;
-      if (p.post) p.grad_post[col] = one_gate ? s * value(p.gate) : s;
-      if (one_gate) p.grad_gate[col] = p.post ? s * value(p.post) : s;
+      if (p.post) (one_gate ? s * value(p.gate) : s).store(p.grad_post + col);
+      if (one_gate) (p.post ? s * value(p.post) : s).store(p.grad_gate + col);
     }
     return;
   }
@@ -847,23 +903,26 @@ __global__ void __launch_bounds__(SUMS_RUNS * 32, 2) norm_sums_kernel(const Norm
     const int runs = p.sums_runs, at = run * p.sums_per >> 16, part = run - at * runs;
     const int g = (GATES == 2 ? (which - 2) * SUMS_RUNS : 0) + at, n = p.ctas_per_gate;
     const bool mine = there && g < p.gates;
-    float s = mine ? sum_run(from + (long long)g * n * p.D, n, part, p.sums_per, p.D, one) : 0.f;
+    Cols<C> s;
+    s.set(0.f);
+    if (mine) s = sum_run<C>(from + (long long)g * n * p.D, n, part, p.sums_per, p.D, as_is);
     sums[run][lane] = s;
     __syncthreads();
     const bool first = part == 0 && mine;
     if (first) {
 #pragma unroll 12
-      for (int i = 1; i < SUMS_RUNS; ++i) s += i < runs ? sums[run + i < SUMS_RUNS ? run + i : 0][lane] : 0.f;
-      p.grad_gate[(long long)g * p.D + col] = p.post ? s * value(p.post) : s;
+      for (int i = 1; i < SUMS_RUNS; ++i)
+        if (i < runs) s += sums[run + i < SUMS_RUNS ? run + i : 0][lane];
+      (p.post ? s * value(p.post) : s).store(p.grad_gate + (long long)g * p.D + col);
     }
     if (GATES == 2 || !p.post) return;
-    if (first) s *= value(p.gate + g * p.ldg);
+    if (first) s = s * value(p.gate + g * p.ldg);
     __syncthreads();
     if (first) sums[at][lane] = s;
     __syncthreads();
     if (run > 0 || !there) return;
     for (int i = 1; i < p.gates; ++i) s += sums[i][lane];
-    p.grad_post[col] = s;
+    s.store(p.grad_post + col);
   }
 }
 
@@ -958,6 +1017,13 @@ static cudaError_t backward_rows(const NormBackwardParams& p, cudaStream_t strea
   if (e != cudaSuccess) return e;
   return launch_behind(norm_backward_kernel<ACT, F32, V>, dim3((unsigned)p.grid, 1, 1), p.threads, p.smem, stream, p);
 }
+template <int ACT, int C>
+static cudaError_t sums_launch(const NormBackwardParams& p, int rows, int kind, cudaStream_t stream) {
+  const dim3 grid((unsigned)((p.D + 32 * C - 1) / (32 * C)), (unsigned)rows, 1);
+  if (kind == 0) return launch_behind(norm_sums_kernel<ACT, 0, C>, grid, SUMS_RUNS * 32, 0, stream, p);
+  if (kind == 1) return launch_behind(norm_sums_kernel<ACT, 1, C>, grid, SUMS_RUNS * 32, 0, stream, p);
+  return launch_behind(norm_sums_kernel<ACT, 2, C>, grid, SUMS_RUNS * 32, 0, stream, p);
+}
 template <int ACT, bool F32>
 static cudaError_t backward_type(NormBackwardParams p, cudaStream_t stream) {
   p.sums_runs = p.gates < SUMS_RUNS ? SUMS_RUNS / p.gates : 1;
@@ -972,10 +1038,8 @@ static cudaError_t backward_type(NormBackwardParams p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const bool shared = p.ctas_per_gate > 1;
   const int post = p.post || (shared && p.grad_gate) ? 2 : 1, more = (p.gates + SUMS_RUNS - 1) / SUMS_RUNS;
-  const dim3 grid((unsigned)((p.D + 31) / 32), (unsigned)(shared && p.gates > SUMS_RUNS ? 2 + more : post), 1);
-  if (!shared || p.gates == 1) return launch_behind(norm_sums_kernel<ACT, 0>, grid, SUMS_RUNS * 32, 0, stream, p);
-  if (p.gates <= SUMS_RUNS) return launch_behind(norm_sums_kernel<ACT, 1>, grid, SUMS_RUNS * 32, 0, stream, p);
-  return launch_behind(norm_sums_kernel<ACT, 2>, grid, SUMS_RUNS * 32, 0, stream, p);
+  const int rows = shared && p.gates > SUMS_RUNS ? 2 + more : post, kind = !shared || p.gates == 1 ? 0 : p.gates <= SUMS_RUNS ? 1 : 2;
+  return p.D > 4096 ? sums_launch<ACT, 2>(p, rows, kind, stream) : sums_launch<ACT, 1>(p, rows, kind, stream);
 }
 // The shape of the gradient's launch: threads and vectors of a row, CTAs (512 threads to an SM), and stages for the rows ahead.
 void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gate, int sms, int max_smem, NormBackwardParams* p) {
