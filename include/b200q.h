@@ -317,14 +317,16 @@ int b200q_gemm_swiglu_cast(const void* a, int lda, const void* bq, const void* s
  *
  * b200q_igemm_plan names the kernel these calls take; b200q_igemm_planned runs an edited plan.  `workspace` holds the
  * status header (256 bytes, zeroed once, as for the other calls of the stream).  The kernels set up under the end of
- * the stream's previous kernel.  With early_b they may read B then: B must not be that kernel's output (weights are not;
- * codes from a cast right in front of the call are).  Everything else, and with early_b 0 B too, is read after it has ended. */
+ * the stream's previous kernel.  With early_b they may read B then: B must have been complete when that kernel started.  (Weights
+ * are; what a cast has written is once a call of this section or the next stands between.  b200q_gemm and its like start their
+ * successor before their predecessor has ended: they do not count.)  Everything else, and with early_b 0 B too, is read after the
+ * previous kernel has ended. */
 typedef struct b200q_igemm_plan {
   int32_t kernel;  /* 1: pairs of CTAs, tiles of 256 rows; 2: all rows against a share of the columns in each CTA (M <= 256);
                       3: mma.sync, B straight from memory (M <= 16) */
   int32_t rows;    /* kernel 2: M rounded up to 16 (output only) */
   int32_t width;   /* kernel 1: product columns of a tile, 256 or 128 (gated: half as many outputs); kernel 2: output columns of
-                      a cluster, the others being of 8 less, a multiple of 8 up to 256 (gated: 128) */
+                      the widest clusters, the others having 8 less; a multiple of 8 up to 256 (gated: 128) */
   int32_t cluster; /* kernel 2: CTAs that share the K of their columns, 1 .. 8 */
   int32_t stages;  /* kernel 2: ring slots of 128 bytes of K, 1 .. 16 */
   int32_t ctas;    /* kernel 1: CTAs, even; kernel 3: CTAs; kernel 2: clusters * cluster; where they are
