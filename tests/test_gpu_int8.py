@@ -9,7 +9,8 @@ import pytest
 import torch
 
 from tests.launches import launches
-from tilus_b200 import Int8Linear, _lib, ops
+from tilus_b200 import Int8Linear, QuantizedLinear, _lib, ops
+from tilus_b200 import dtypes as D
 
 pytestmark = pytest.mark.gpu
 F64 = torch.float64
@@ -296,6 +297,27 @@ def test_operands_that_other_kernels_write_right_before(M):
         for dst, src in zip((a, a_sf, b_sf, b), others[i % 2][:1] + others[i % 2][2:] + others[i % 2][1:2]):
             dst.copy_(src)
         assert torch.equal(ops.int8_matmul(a, b, a_sf, b_sf), wants[i % 2])
+
+
+@pytest.mark.parametrize("M", [1, 40])
+def test_weights_cast_in_front_of_a_product_that_starts_its_successor_early(M):
+    """Between the cast and the product a weight-only product runs, which lets its successor start before the cast has ended."""
+    torch.manual_seed(6)
+    w = torch.randn(8192, 2048, device="cuda").half()
+    x, x_sf = ops.per_token_cast_int8(torch.randn(M, 2048, device="cuda").half())
+    between = QuantizedLinear("float16", D.int4b, 128, 1024, 1024).cuda()
+    small = torch.randn(16, 1024, device="cuda").half()
+    want = []
+    for sign in (1, -1):
+        c, sf = ops.per_token_cast_int8(sign * w)
+        torch.cuda.synchronize()
+        want.append(ops.int8_matmul(x, c, x_sf, sf))
+    between(small)
+    torch.cuda.synchronize()
+    for i in range(20):
+        c, sf = ops.per_token_cast_int8(w if i % 2 == 0 else -w)
+        between(small)
+        assert torch.equal(ops.int8_matmul(x, c, x_sf, sf), want[i % 2])
 
 
 def test_codes_of_a_norm_as_weights():
