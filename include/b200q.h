@@ -317,10 +317,10 @@ int b200q_gemm_swiglu_cast(const void* a, int lda, const void* bq, const void* s
  *
  * b200q_igemm_plan names the kernel these calls take; b200q_igemm_planned runs an edited plan.  `workspace` holds the
  * status header (256 bytes, zeroed once, as for the other calls of the stream).  The kernels set up under the end of
- * the stream's previous kernel.  With early_b they may read B then: B must have been complete when that kernel started.  (Weights
- * are; what a cast has written is once a call of this section or the next stands between.  b200q_gemm and its like start their
+ * the stream's previous kernel.  With early_b they may read B then: B must have been complete when that kernel started.  (What any
+ * kernel has written is once a call of this section or the next stands between.  b200q_gemm and its like start their
  * successor before their predecessor has ended: they do not count.)  Everything else, and with early_b 0 B too, is read after the
- * previous kernel has ended. */
+ * previous kernel has ended; rows of B may be brought into L2 before. */
 typedef struct b200q_igemm_plan {
   int32_t kernel;  /* 1: pairs of CTAs, tiles of 256 rows; 2: all rows against a share of the columns in each CTA (M <= 256);
                       3: mma.sync, B straight from memory (M <= 16) */

@@ -22,7 +22,7 @@ struct Int8Params {
   int tiles, m_tiles, n_tiles, m_group;  // pair kernel: output tiles and their raster groups
   int rows, width, wide;       // stream kernel: rows of A rounded up to 16; output columns of the first `wide` CTAs (or clusters)
   int cluster, stages, smem;   // CTAs that share K, ring slots, dynamic shared memory
-  int early;                   // stream and row kernels: the kernel before this one does not write B
+  int early;                   // stream and row kernels: B was complete when the kernel before this one started
 };
 
 // api.cu

@@ -22,7 +22,8 @@
 // 8192 23.6 us (5.7 TB/s), 64 x 28672 x 4096 gated 21.4 us; row, 1 x 4096 x 4096 3.6 us.
 //
 // All are launched with programmatic stream serialization: they set up under the end of the kernel before them.  All they read
-// before that kernel has ended is, in the stream and row kernels and where the caller says that it may (`early`), rows of B.  Like the
+// before that kernel has ended is, in the stream and row kernels and where the caller says that it may (`early`), rows of B; the
+// stream kernel asks for them in L2 otherwise, which reads no value.  Like the
 // row-wise kernels they let the kernel behind them start only after their own wait, so that whatever runs then, the kernel
 // before the last has ended; and only once they have their tensor memory, which a CTA behind them, waiting for their end, could
 // otherwise hold.
@@ -398,6 +399,12 @@ __device__ __forceinline__ void stream_load_b(const Int8Params& p, const CUtenso
         ::"r"(dst + (uint32_t)(h * width) * 128u), "l"(tb), "r"(bar), "r"(kb * 128), "r"(n0 + h * p.N) : "memory");
 }
 
+// The same rows into L2 only.
+__device__ __forceinline__ void stream_prefetch_b(const Int8Params& p, const CUtensorMap* tb, bool gated, int kb, int n0) {
+  for (int h = 0; h < (gated ? 2 : 1); ++h)
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tb), "r"(kb * 128), "r"(n0 + h * p.N) : "memory");
+}
+
 template <bool GATED>
 __global__ void __launch_bounds__(S_THREADS)
     int8_stream_kernel(const Int8Params p, const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
@@ -444,11 +451,16 @@ __global__ void __launch_bounds__(S_THREADS)
 
   if (warp < S_COPIERS) {
     if (elect_one()) {
-      if (p.early)  // rows of B, which the kernel before this one does not write: the first of them come under its end
+      // The first rows of B come under the end of the kernel before this one: into shared memory where the caller says that B has been
+      // complete since before that kernel, else as far as L2, where what that kernel still writes meets them.  (us, read early / into
+      // L2 / neither: 8 x 28672 x 4096 gated 37.5 / 37.9 / 39.1, 64 x 14336 x 4096 gated 21.2 / 21.5 / 22.1.)
+      if (p.early)
         for (int i = warp; i < p.stages && kb0 + i < kb1; i += S_COPIERS) {
           expect_bytes(BAR(full, i), stage_bytes);
           stream_load_b(p, map_b, GATED, ring + (uint32_t)i * stage_bytes, BAR(full, i), kb0 + i, n0, width);
         }
+      else
+        for (int i = warp; i < p.stages && kb0 + i < kb1; i += S_COPIERS) stream_prefetch_b(p, map_b, GATED, kb0 + i, n0);
       asm volatile("prefetch.tensormap [%0];" ::"l"(&ta) : "memory");
     }
     __syncwarp();

@@ -84,7 +84,6 @@ struct StreamBuffers {
   at::Tensor workspace;
   at::Tensor staging[2][2];
   std::vector<at::Tensor> superseded;
-  const char *cast_begin = nullptr, *cast_end = nullptr;  // codes that the stream's latest cast writes, see codes_written
   std::mutex host_call;  // a host call is several operations on one staging pair: one thread's at a time
 };
 std::mutex g_mutex;
@@ -424,28 +423,6 @@ bool optional_tensor(PyObject* o, const char* name, const at::Tensor** t) {
   return *t != nullptr;
 }
 
-// A product may read its operand B (weights) before the kernel in front of it has ended, unless that one writes it.  What writes
-// int8 codes here are the casts, and each kernel of these operators lets the next one start only when the one before itself has
-// ended: so it is a stream's latest cast that matters.  Its outputs are noted until a product has been launched behind it (which
-// waits for it and for everything before).  Other streams' latest casts count too: in a capture that joins streams the product's edge
-// from each kernel that it follows may be one that lets it set up early.
-void codes_written(int device, cudaStream_t stream, const void* codes, int64_t bytes) {
-  std::lock_guard<std::mutex> lock(g_mutex);
-  StreamBuffers& b = buffers_of(device, stream);
-  b.cast_begin = static_cast<const char*>(codes);
-  b.cast_end = b.cast_begin + bytes;
-}
-bool settled(int device, cudaStream_t stream, const void* operand, int64_t bytes) {
-  std::lock_guard<std::mutex> lock(g_mutex);
-  const char* p = static_cast<const char*>(operand);
-  bool apart = true;
-  for (const auto& b : pool()) {
-    if (b->device == device && b->cast_begin && p < b->cast_end && p + bytes > b->cast_begin) apart = false;
-    if (b->device == device && b->stream == stream) b->cast_begin = b->cast_end = nullptr;
-  }
-  return apart;
-}
-
 // cast_int8(x) -> (out int8 [tokens, hidden], out_sf float32 [tokens])
 PyObject* cast_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -464,7 +441,6 @@ PyObject* cast_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const void* xp = x->const_data_ptr();
     void *op = out.mutable_data_ptr(), *fp = sf.mutable_data_ptr();
     const int ldx = (int)row_stride(*x);
-    codes_written(dev.index(), stream, op, (int64_t)T * H);
     int st;
     {
       const NoGil unlocked;
@@ -476,16 +452,18 @@ PyObject* cast_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// igemm(a, b, a_sf, b_sf, bias or None, activation type's code, gated, clamp value or None, out or None) -> out
+// igemm(a, b, a_sf, b_sf, bias or None, activation type's code, gated, clamp value or None, out or None, early) -> out
+// `early`: the caller knows that B has been complete since before the stream's previous kernel.  (Nothing here can know it: kernels of others
+// are not seen, and what a kernel has written that lets its successor start under its end counts only after that successor's wait.)
 PyObject* igemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 9) { type_error("igemm takes 9 arguments"); return nullptr; }
+  if (nargs != 10) { type_error("igemm takes 10 arguments"); return nullptr; }
   const at::Tensor *a = as_tensor(args[0], "a"), *b = a ? as_tensor(args[1], "b") : nullptr;
   const at::Tensor *a_sf = b ? as_tensor(args[2], "a_sf") : nullptr, *b_sf = a_sf ? as_tensor(args[3], "b_sf") : nullptr;
   const at::Tensor *bias, *given;
   if (!b_sf || !optional_tensor(args[4], "bias", &bias) || !optional_tensor(args[8], "out", &given)) return nullptr;
   const long act = PyLong_AsLong(args[5]);
-  const int gated = PyObject_IsTrue(args[6]);
+  const int gated = PyObject_IsTrue(args[6]), early = PyObject_IsTrue(args[9]);
   const bool clamp = args[7] != Py_None;
   const double clamp_value = clamp ? PyFloat_AsDouble(args[7]) : 0.0;
   if (PyErr_Occurred()) return nullptr;
@@ -516,7 +494,6 @@ PyObject* igemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     void *c = out.mutable_data_ptr(), *w = ws.mutable_data_ptr();
     const int lda = (int)row_stride(*a), ldb = (int)row_stride(*b), ldc = (int)row_stride(out);
     const size_t ws_bytes = (size_t)ws.numel();
-    const int early = settled(dev.index(), stream, bp, (rows - 1) * ldb + K) ? 1 : 0;
     int st;
     {
       const NoGil unlocked;
@@ -602,7 +579,6 @@ PyObject* block_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (T > 0) {
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
     void *xp = x.mutable_data_ptr(), *rp = fresh.mutable_data_ptr(), *fp = cast ? sf.mutable_data_ptr() : nullptr;
-    if (cast) codes_written(dev.index(), stream, xp, T * D);
     int st;
     {
       const NoGil unlocked;

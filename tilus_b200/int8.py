@@ -73,25 +73,33 @@ class Int8Linear(nn.Module):
         """x [..., in_features] in the activations' type: cast per token, then multiplied."""
         if x.dtype != self.act_torch_dtype:
             raise TypeError(f"activations must be {self.act_torch_dtype}")
-        out = self.forward_cast(*ops.per_token_cast_int8(self._rows(x)))
+        weight, rest = self.weight, dict(bias=self.bias, out_dtype=self.act_torch_dtype)
+        # (early: the cast behind all that wrote the weights, which may be a parametrization just now, waits for it)
+        codes, x_sf = ops.per_token_cast_int8(self._rows(x))
+        out = ops.int8_matmul(codes, weight, x_sf, self.scales, early_b=True, **rest)
         return out if x.dim() == 2 else out.reshape(*x.shape[:-1], self.out_features)
 
-    def forward_cast(self, x: torch.Tensor, x_sf: torch.Tensor) -> torch.Tensor:
+    def forward_cast(self, x: torch.Tensor, x_sf: torch.Tensor, *, early_b: bool = False) -> torch.Tensor:
         """forward() for activations that are cast already (int8 [tokens, in_features], float32 [tokens]), by
-        per_token_cast_int8 or block_norm_cast_int8."""
-        return ops.int8_matmul(x, self.weight, x_sf, self.scales, bias=self.bias, out_dtype=self.act_torch_dtype)
+        per_token_cast_int8 or block_norm_cast_int8.  ``early_b`` as for ops.int8_matmul: where that cast or norm stands
+        directly in front and the weights (parameters, not computed on access) were written before it."""
+        return ops.int8_matmul(x, self.weight, x_sf, self.scales, bias=self.bias, out_dtype=self.act_torch_dtype,
+                               early_b=early_b)
 
-    def forward_swiglu(self, x: torch.Tensor, x_sf: torch.Tensor | None = None, swiglu_clamp_value=None) -> torch.Tensor:
+    def forward_swiglu(self, x: torch.Tensor, x_sf: torch.Tensor | None = None, swiglu_clamp_value=None, *,
+                       early_b: bool = False) -> torch.Tensor:
         """For a gate_up projection (out_features = 2 * hidden, gate rows first): silu(gate) * up [tokens, hidden] from one
-        kernel.  ``x`` as forward() takes it, or with ``x_sf`` as forward_cast() does."""
+        kernel.  ``x`` as forward() takes it, or with ``x_sf`` (and ``early_b``) as forward_cast() does."""
         if self.bias is not None:
             raise ValueError("a gate_up projection has no bias here")
+        weight = self.weight
         if x_sf is None:
             if x.dtype != self.act_torch_dtype:
                 raise TypeError(f"activations must be {self.act_torch_dtype}")
             x, x_sf = ops.per_token_cast_int8(self._rows(x))
-        return ops.int8_gate_up(x, self.weight, x_sf, self.scales, out_dtype=self.act_torch_dtype,
-                                swiglu_clamp_value=swiglu_clamp_value)
+            early_b = True  # as in forward()
+        return ops.int8_gate_up(x, weight, x_sf, self.scales, out_dtype=self.act_torch_dtype,
+                                swiglu_clamp_value=swiglu_clamp_value, early_b=early_b)
 
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, x_dtype={self.x_dtype.name}, "

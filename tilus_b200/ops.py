@@ -188,20 +188,25 @@ def per_token_cast_int8(x: torch.Tensor):
 
 
 def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_sf: torch.Tensor, b_sf: torch.Tensor, bias: torch.Tensor | None = None,
-                out_dtype: torch.dtype = torch.float16, out: torch.Tensor | None = None) -> torch.Tensor:
+                out_dtype: torch.dtype = torch.float16, out: torch.Tensor | None = None, *, early_b: bool = False) -> torch.Tensor:
     """C[M, N] = (A x B^T) * a_sf[:, None] * b_sf + bias for int8 ``a`` [M, K] and ``b`` [N, K] with float32 scales per
     row of A (token) and per row of B (channel).  The sums are exact (int32); C and ``bias`` are float16 or bfloat16.
-    N and K are multiples of 16, K at most 131056; rows may be strided (by multiples of 16 bytes)."""
-    return _lib.native().igemm(a, b, a_sf, b_sf, bias, act_code(out_dtype), False, None, out)
+    N and K are multiples of 16, K at most 131056; rows may be strided (by multiples of 16 bytes).
+
+    ``early_b``: ``b`` may be read while the stream's previous kernel still runs.  Say so only where ``b`` was complete
+    before that kernel started: weights at rest, with a cast, norm or product of this library between what wrote them (on any
+    stream) and this call.  It saves a small product up to 1 us."""
+    return _lib.native().igemm(a, b, a_sf, b_sf, bias, act_code(out_dtype), False, None, out, early_b)
 
 
 def int8_gate_up(a: torch.Tensor, b: torch.Tensor, a_sf: torch.Tensor, b_sf: torch.Tensor,
                  out_dtype: torch.dtype = torch.float16, swiglu_clamp_value=None,
-                 out: torch.Tensor | None = None) -> torch.Tensor:
+                 out: torch.Tensor | None = None, *, early_b: bool = False) -> torch.Tensor:
     """A gate_up projection in 8-bit integers with its SwiGLU, in one kernel: ``b`` [2 * hidden, K] holds the gate's rows
     first; returns silu(gate) * up [M, hidden], clamped as swiglu_forward_and_per_token_cast does where
-    ``swiglu_clamp_value`` is given.  Neither projection is written to memory or rounded on its way."""
-    return _lib.native().igemm(a, b, a_sf, b_sf, None, act_code(out_dtype), True, swiglu_clamp_value, out)
+    ``swiglu_clamp_value`` is given.  Neither projection is written to memory or rounded on its way.  ``early_b`` as for
+    int8_matmul."""
+    return _lib.native().igemm(a, b, a_sf, b_sf, None, act_code(out_dtype), True, swiglu_clamp_value, out, early_b)
 
 
 def int8_plan(M: int, N: int, K: int, gated: bool = False) -> dict:
