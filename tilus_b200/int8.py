@@ -11,6 +11,7 @@ from torch import nn
 
 from . import ops
 from .dtypes import act_dtype
+from .grad import followed, without_backward
 
 _TORCH_ACT = {"float16": torch.float16, "bfloat16": torch.bfloat16}
 
@@ -23,7 +24,8 @@ class Int8Linear(nn.Module):
           .scales : float32[out_features]
           .bias   : x_dtype[out_features] or None
 
-    in_features and out_features are multiples of 16.  The forward passes run the CUDA library; there is no CPU path."""
+    in_features and out_features are multiples of 16.  The forward passes run the CUDA library; there is no CPU path.  They have
+    no backward pass: where activations require a gradient, backward() through the result raises."""
 
     def __init__(self, x_dtype, in_features: int, out_features: int, bias: bool = False):
         super().__init__()
@@ -71,6 +73,8 @@ class Int8Linear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """x [..., in_features] in the activations' type: cast per token, then multiplied."""
+        if followed(x):
+            return without_backward("Int8Linear", self.forward, x)
         if x.dtype != self.act_torch_dtype:
             raise TypeError(f"activations must be {self.act_torch_dtype}")
         weight, rest = self.weight, dict(bias=self.bias, out_dtype=self.act_torch_dtype)
@@ -92,6 +96,8 @@ class Int8Linear(nn.Module):
         kernel.  ``x`` as forward() takes it, or with ``x_sf`` (and ``early_b``) as forward_cast() does."""
         if self.bias is not None:
             raise ValueError("a gate_up projection has no bias here")
+        if followed(x):
+            return without_backward("Int8Linear", lambda t: self.forward_swiglu(t, x_sf, swiglu_clamp_value, early_b=early_b), x)
         weight = self.weight
         if x_sf is None:
             if x.dtype != self.act_torch_dtype:

@@ -21,6 +21,7 @@ from torch import nn
 from . import ops, packing, quantize
 from ._lib import native
 from .dtypes import KIND_UINT, act_dtype, weight_dtype
+from .grad import without_backward
 
 _TORCH_ACT = {"float16": torch.float16, "bfloat16": torch.bfloat16}
 
@@ -154,6 +155,10 @@ class QuantizedLinear(nn.Module):
         return qw, scales, (self.w_dtype.code, self.zero_point, self.group_size, self.in_features, self.out_features)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """x [..., in_features] -> [..., out_features].  There is no backward pass: where ``x`` requires a gradient, backward()
+        through the result raises."""
+        if torch.is_grad_enabled() and getattr(x, "requires_grad", False):
+            return without_backward("QuantizedLinear", lambda t: native().linear(t, *self._operands()), x)
         return native().linear(x, *self._operands())
 
     def forward_host(self, x_host: torch.Tensor, out_host: torch.Tensor | None = None) -> torch.Tensor:

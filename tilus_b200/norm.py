@@ -1,7 +1,7 @@
 """BlockNorm: the norms before and after a decoder block with its gate and residual scale, as a module.
 
 ops.block_norm and ops.block_norm_backward are the operators; this module holds their weights and ties them together for
-autograd (norm weights and gates are what is tuned after a model's linears are quantized).
+autograd.  The layers of this package have no backward pass: gradients come as far as the norms that no such layer stands behind.
 """
 from __future__ import annotations
 
@@ -10,6 +10,7 @@ from torch import nn
 
 from . import ops
 from .dtypes import act_dtype
+from .grad import followed
 
 _TORCH_ACT = {"float16": torch.float16, "bfloat16": torch.bfloat16}
 
@@ -43,13 +44,16 @@ def _rows(grad: torch.Tensor) -> torch.Tensor:
 
 
 def block_norm(block, residual, weight, *, post_weight=None, gate=None, residual_scale=1.0, eps=1e-6):
-    """ops.block_norm as a differentiable function.  Not for stream capture while gradients are recorded: autograd's own
-    bookkeeping outlives a capture; capture ops.block_norm and ops.block_norm_backward instead."""
+    """ops.block_norm as a function of torch's autograd (backward only; tangents are refused).  Not for stream capture while gradients
+    are recorded: autograd's own bookkeeping outlives a capture; capture ops.block_norm and ops.block_norm_backward instead."""
     operands = (block, residual, weight, post_weight, gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
-        if block.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("block_norm records gradients and cannot be captured: capture ops.block_norm and "
-                               "ops.block_norm_backward, or capture under torch.no_grad()")
+    if followed(*operands):
+        if block.is_cuda:
+            with torch.cuda.device(block.device):
+                capturing = torch.cuda.is_current_stream_capturing()
+            if capturing:
+                raise RuntimeError("block_norm records gradients and cannot be captured: capture ops.block_norm and "
+                                   "ops.block_norm_backward, or capture under torch.no_grad()")
         return _BlockNorm.apply(*operands, residual_scale, eps)
     return ops.block_norm(block, residual, weight, post_weight=post_weight, gate=gate, residual_scale=residual_scale, eps=eps)
 

@@ -181,8 +181,8 @@ def swiglu_forward_and_per_token_cast(x: torch.Tensor, num_per_channels: int = 1
 # ---- 8-bit integers on both sides ----------------------------------------------------------------------
 def per_token_cast_int8(x: torch.Tensor):
     """x [tokens, hidden] (float16 / bfloat16, CUDA; hidden a multiple of 8) -> (out int8 [tokens, hidden], out_sf float32
-    [tokens]): codes of largest magnitude 127, and the scale that a code stands for.  Activations are cast a row a token,
-    weights [out_features, in_features] a row a channel.  A row of zeros has scale 1; a row with a NaN or an infinity
+    [tokens]): codes of largest magnitude 127, and the scale that a code stands for (no gradients).  Activations are cast a row
+    a token, weights [out_features, in_features] a row a channel.  A row of zeros has scale 1; a row with a NaN or an infinity
     has it as its scale, so that products with it are NaN."""
     return _lib.native().cast_int8(x)
 
@@ -229,7 +229,8 @@ def block_norm(block: torch.Tensor, residual: torch.Tensor | None, weight: torch
     Returns (x, new_residual): the next block's input in the type of ``block`` (float16 / bfloat16) and the residual
     stream in its own type, which is that or float32.  ``gate`` is [hidden], or [gates, hidden] with a row for each run of
     tokens / gates rows (one for each sequence of a batch).  hidden is a multiple of 8, at most 16384.  All sums are
-    float32, and x comes from the residual before it is rounded."""
+    float32, and x comes from the residual before it is rounded.  Autograd does not see this call; norm.block_norm is the
+    differentiable one."""
     return _lib.native().block_norm(block, residual, weight, post_weight, gate, residual_scale, eps, False)
 
 
