@@ -225,3 +225,27 @@ def test_between_a_weight_only_product_and_a_cast():
     torch.cuda.synchronize()
     for _ in range(20):
         assert torch.equal(second(first(x)), want)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_an_output_that_autograd_has_saved(gated):
+    """Writing to `out` counts as a change of it, and it must not want a gradient itself."""
+    a, b, a_sf, b_sf = _operands(4, 64, 128)
+    call = ops.int8_gate_up if gated else ops.int8_matmul
+    out = call(a, b, a_sf, b_sf)
+    weight = torch.ones_like(out, requires_grad=True)
+    y = (out * weight).sum()
+    before = out._version
+    call(a, b, a_sf, b_sf, out=out)
+    after = out._version
+    assert after > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with pytest.raises(ValueError, match="must not require a gradient"):
+        call(a, b, a_sf, b_sf, out=weight)
+    with torch.no_grad():
+        call(a, b, a_sf, b_sf, out=weight)
+    with torch.inference_mode():
+        static = call(a, b, a_sf, b_sf)
+        call(a, b, a_sf, b_sf, out=static)
+    assert torch.equal(weight, static) and torch.equal(out, static)

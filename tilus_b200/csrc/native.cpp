@@ -11,6 +11,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -482,6 +483,7 @@ PyObject* igemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!check_rows(*given, "out", dev)) return nullptr;
     if (given->scalar_type() != type) { type_error("out must be of out_dtype"); return nullptr; }
     if (given->size(0) != M || given->size(1) != N) { value_error("out has the wrong shape"); return nullptr; }
+    if (c10::GradMode::is_enabled() && given->requires_grad()) { value_error("out must not require a gradient"); return nullptr; }
   }
   at::Tensor out;
   if (given) out = *given;
@@ -502,6 +504,7 @@ PyObject* igemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                  : g_igemm(ap, lda, bp, ldb, fa, fb, biasp, c, ldc, (int)M, (int)N, (int)K, (int)act, early, w, ws_bytes, stream);
     }
     if (st != 0) return raise_status(st);
+    if (given && !given->is_inference()) given->unsafeGetTensorImpl()->bump_version();  // autograd may have saved it
   }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS

@@ -191,7 +191,8 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_sf: torch.Tensor, b_sf: torc
                 out_dtype: torch.dtype = torch.float16, out: torch.Tensor | None = None, *, early_b: bool = False) -> torch.Tensor:
     """C[M, N] = (A x B^T) * a_sf[:, None] * b_sf + bias for int8 ``a`` [M, K] and ``b`` [N, K] with float32 scales per
     row of A (token) and per row of B (channel).  The sums are exact (int32); C and ``bias`` are float16 or bfloat16.
-    N and K are multiples of 16, K at most 131056; rows may be strided (by multiples of 16 bytes).
+    N and K are multiples of 16, K at most 131056; rows may be strided (by multiples of 16 bytes).  Autograd does not see
+    this call; ``out`` is a tensor without a gradient.
 
     ``early_b``: ``b`` may be read while the stream's previous kernel still runs.  Say so only where ``b`` was complete
     before that kernel started: weights at rest, with a cast, norm or product of this library between what wrote them (on any
