@@ -49,6 +49,9 @@ __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {  // a
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+__device__ __forceinline__ void store_peer(uint32_t addr, int v) {  // to an address of map_to
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -114,7 +117,8 @@ constexpr int P_THREADS = 128 + P_WRITERS;  // copies of A, products, tensor mem
 struct PairBars {
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, peer_abort;
+  int issued[4];  // pieces that the copying warps have asked for: of A and of B, and in the first CTA the second one's
 };
 constexpr int P_SCALES = 256 * 4 + 256 * 2;  // a tile's column scales and biases
 int int8_pair_smem_bytes(int cols) {
@@ -154,7 +158,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) { mbar_init(BAR(full, i), 1); mbar_init(BAR(empty, i), 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(BAR(acc_full, i), 1); mbar_init(BAR(acc_empty, i), 2 * (P_WRITERS / 32)); }
-    bars->abort_flag = 0;
+    bars->abort_flag = bars->peer_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -195,11 +199,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
           if (++s == STAGES) { s = 0; phase ^= 1u; }
         }
       }
-      // Having given up: the copies in flight land before the CTA ends (both CTAs' count on the first one's barriers, and the
-      // second CTA waits for the first at the end).
-      if (*abort_flag && rank == 0 && warp == 0) ring_drain(BAR(full, 0), STAGES, issued);
-      if (*abort_flag && warp == 3)  // (rows of B may have been asked for that the first CTA counts no rows of A with)
-        for (const long long t0 = clock64(); clock64() - t0 < 200000;) {}
+      bars->issued[warp == 0 ? 0 : 1] = issued;
     }
   } else if (warp == 1) {
     // ---- products, issued by the first CTA for both ----
@@ -343,8 +343,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     p.status[1] = 12;  // where: pair kernel
     p.status[2] = blockIdx.x;
     p.status[3] = 0;
+    store_peer(map_to(bars_s + (uint32_t)offsetof(PairBars, peer_abort), rank ^ 1u), 1);
   }
   cluster_sync();  // neither CTA's shared memory or tensor memory goes while the other still uses it
+  if (*abort_flag || *static_cast<volatile int*>(&bars->peer_abort)) {
+    // One of the two has given up (both see it): the copies in flight, which all report to the first CTA, land before the CTAs end.
+    if (rank == 1 && tid < 2) store_peer(map_to(bars_s + (uint32_t)offsetof(PairBars, issued) + (uint32_t)(2 + tid) * 4u, 0), bars->issued[tid]);
+    __syncwarp();
+    cluster_sync();
+    if (rank == 0 && tid < STAGES) {
+      const int issued[4] = {bars->issued[0], bars->issued[1], bars->issued[2], bars->issued[3]};
+      const uint32_t bytes[4] = {16384u, STAGE - 16384u, 16384u, STAGE - 16384u};
+      const RingRest rest = ring_rest(tid, STAGES, issued, bytes);
+      if (rest.announce) expect_bytes(BAR(full, tid), rest.announce);
+      if (rest.strike)
+        asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(BAR(full, tid)), "r"(rest.strike) : "memory");
+      if (rest.item >= 0) mbar_wait_bounded(BAR(full, tid), (uint32_t)(rest.item / STAGES) & 1u);
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 2) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
