@@ -467,11 +467,13 @@ __global__ void __launch_bounds__(S_THREADS)
   // every CTA of the cluster runs before its shared memory is written (waited for at the first store)
   if (S > 1 && apart) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
+  bool copies = false;   // this thread's, and how far they are: the next slot, and how often the ring has been gone round
+  int slot = warp, lap = 0;
   if (warp < S_COPIERS) {
     if (elect_one()) {
       // The first rows of B come under the end of the kernel before this one: into shared memory where the caller says that B has been
       // complete since before that kernel, else as far as L2, where what that kernel still writes meets them.  (us, read early / into
-      // L2 / neither: 8 x 28672 x 4096 gated 37.5 / 37.9 / 39.1, 64 x 14336 x 4096 gated 21.2 / 21.5 / 22.1.)
+      // L2 / neither: 8 x 57344 x 4096 gated 37.5 / 37.9 / 39.1, 64 x 28672 x 4096 gated 21.2 / 21.5 / 22.1.)
       if (p.early)
         for (int i = warp; i < p.stages && kb0 + i < kb1; i += S_COPIERS) {
           expect_bytes(BAR(full, i), stage_bytes);
@@ -484,12 +486,12 @@ __global__ void __launch_bounds__(S_THREADS)
     __syncwarp();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (elect_one()) {
-      // Block kb0 + lap * stages + s goes to slot s, and a slot is one warp's: a wait for its barrier's parity is then never more than
-      // a phase behind.
-      int s = warp, lap = 0;
-      for (int kb = kb0 + warp; s < p.stages && kb < kb1; kb = kb0 + lap * p.stages + s) {
-        if (!mbar_wait_abortable(BAR(empty, s), ((uint32_t)lap & 1u) ^ 1u, abort_flag)) break;
-        const uint32_t bar = BAR(full, s), dst = ring + (uint32_t)s * stage_bytes;
+      // Block kb0 + lap * stages + slot goes to slot `slot`, and a slot is one warp's: a wait for its barrier's parity is then never more
+      // than a phase behind.
+      copies = true;
+      for (int kb = kb0 + warp; slot < p.stages && kb < kb1; kb = kb0 + lap * p.stages + slot) {
+        if (!mbar_wait_abortable(BAR(empty, slot), ((uint32_t)lap & 1u) ^ 1u, abort_flag)) break;
+        const uint32_t bar = BAR(full, slot), dst = ring + (uint32_t)slot * stage_bytes;
         if (!p.early || lap > 0) {
           expect_bytes(bar, stage_bytes);
           stream_load_b(p, map_b, GATED, dst, bar, kb, n0, width);
@@ -497,14 +499,9 @@ __global__ void __launch_bounds__(S_THREADS)
         asm volatile(
             "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
             ::"r"(dst + b_bytes), "l"(&ta), "r"(bar), "r"(kb * 128), "r"(0) : "memory");
-        s += S_COPIERS;
-        if (s >= p.stages) { s = warp; ++lap; }
+        slot += S_COPIERS;
+        if (slot >= p.stages) { slot = warp; ++lap; }
       }
-      if (*abort_flag)  // the copies in flight land before the CTA ends: the last of each slot
-        for (int q = warp; q < p.stages; q += S_COPIERS) {
-          const int last = q < s ? lap : lap - 1;
-          if (last >= 0 && kb0 + last * p.stages + q < kb1) mbar_wait_bounded(BAR(full, q), (uint32_t)last & 1u);
-        }
     }
     __syncwarp();
   } else if (warp == S_COPIERS) {
@@ -649,6 +646,12 @@ __global__ void __launch_bounds__(S_THREADS)
     p.status[2] = blockIdx.x;
     p.status[3] = 0;
   }
+  if (*abort_flag && copies)  // the copies in flight land before the CTA ends: the last of each slot
+    for (int q = warp; q < p.stages; q += S_COPIERS) {
+      const int last = q < slot ? lap : lap - 1;
+      if (last >= 0 && kb0 + last * p.stages + q < kb1) mbar_wait_bounded(BAR(full, q), (uint32_t)last & 1u);
+    }
+  __syncwarp();
   if (warp == S_COPIERS) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
