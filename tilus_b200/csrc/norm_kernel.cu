@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
   extern __shared__ __align__(16) unsigned char rows_smem[];  // [stage]: a row of block, grad_x, residual, grad_new
   __shared__ __align__(16) float slots[2][8 * (NORM_BACK_THREADS / 32)], slots_block[1][32];
   __shared__ uint64_t landed[NORM_BACK_STAGES];
-  __shared__ int gave_up;
+  __shared__ int gave_up, run_start, run_asked;  // (the rows of the runs before thread 0's latest, and those of it that it has asked for)
   constexpr int RB = F32 ? 4 : 2;
   constexpr bool KEEP = V <= 2;
   start_behind();
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
     // Thread 0 asks for rows, in order, the stages in turn from this run's first.
     int asked = 0, ask_stage = at;
     auto fetch = [&]() {
-      if (asked >= rows) return;
+      if (asked >= rows || !good) return;  // (once thread 0 has given up, no stage is asked for again)
       const long long t = t0 + asked;
       const uint32_t bar = landed_s + (uint32_t)ask_stage * 8u, to = ring + (uint32_t)ask_stage * stage;
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
@@ -642,18 +642,22 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
       copy_row(to + row16, p.grad_x + t * p.lddx, row16, bar);
       if (p.residual) copy_row(to + 2u * row16, static_cast<const char*>(p.residual) + t * p.ldr * RB, row_wide, bar);
       if (p.grad_new) copy_row(to + 2u * row16 + row_wide, static_cast<const char*>(p.grad_new) + t * p.lddn * RB, row_wide, bar);
-      ++asked;
+      run_asked = ++asked;
       if (++ask_stage == p.stages) ask_stage = 0;
     };
-    // A thread that has given up waits no more, but keeps in step with the others.
+    // A thread that has given up waits no more, but keeps in step with the others; its part of this row's and all later rows'
+    // reductions is no number, and so is what they give: the rows' gradients and the CTA's shares of all sums.
     auto await = [&](int stage_i, int lap_i) {
       if (good && !mbar_wait_bounded(landed_s + (uint32_t)stage_i * 8u, (uint32_t)lap_i & 1u)) {
         good = false;
         gave_up = 1;
       }
     };
-    if (me == 0)
+    if (me == 0 && good) {
+      run_start = lap * p.stages + at;
+      run_asked = 0;
       for (int n = 0; n < p.stages; ++n) fetch();
+    }
     float s1 = 1.f;
     if (ahead && p.post && rows > 0) {
       await(at, lap);
@@ -688,7 +692,7 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
           }
         }
       }
-      float x[8] = {sum(rr), sum(er), sum(qn), sum(qe), sum(qr), 0.f, 0.f, 0.f};
+      float x[8] = {good ? sum(rr) : __int_as_float(0x7fc00000), sum(er), sum(qn), sum(qe), sum(qr), 0.f, 0.f, 0.f};
       if (ahead && p.post && n + 1 < rows) {
         await(next, next_lap);
         x[5] = block_square(ring + (uint32_t)next * stage);
@@ -768,18 +772,14 @@ __global__ void __launch_bounds__(NORM_BACK_THREADS) norm_backward_kernel(const 
     __syncthreads();  // the stages and slots of this run's last row have been read
   }
   if (gave_up) {
-    // The copies in flight get their chance to land before the CTA ends, and the sums are no numbers.
+    // The copies in flight get their chance to land before the CTA ends.
     if (me == 0) {
-      for (int i = 0; i < p.stages; ++i) {
-        const int last = i < at ? lap : lap - 1;
-        if (last >= 0) mbar_wait_bounded(landed_s + (uint32_t)i * 8u, (uint32_t)last & 1u);
-      }
+      ring_drain(landed_s, p.stages, run_start + run_asked);
       atomicExch(p.status, ST_DEVICE_TIMEOUT);
       p.status[1] = 14;  // where: gradient of the block norm
       p.status[2] = blockIdx.x;
       p.status[3] = 0;
     }
-    gw[0][0] = both(__int_as_float(0x7fc00000));
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
