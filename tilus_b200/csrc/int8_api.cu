@@ -22,21 +22,19 @@ static int check_igemm(int M, int N, int K) {
 }
 static int igemm_kblocks(int K) { return (K + 127) / 128; }
 
-static int pair_tiles(int M, int N, bool gated, int cols) {
-  const int per = gated ? cols / 2 : cols;
-  return (int)(((long long)M + 255) / 256 * ((N + per - 1) / per));
-}
+static int parts(int n, int of) { return (n - 1) / of + 1; }  // of `of` each that n >= 1 makes (n may be any int)
+static long long pair_tiles(int M, int N, bool gated, int cols) { return (long long)parts(M, 256) * parts(N, gated ? cols / 2 : cols); }
 // Shares of the columns in the stream kernel, of which `at_once` run at once: as many as that in as few rounds as the tensor core's
 // 256 columns allow, but of two units of 8 columns at least.  They differ by a unit at most.  Where an SM
 // has one, as few as have the widest width, since each reads A (64 x 12288 x 4096 11.6 us with 140, 12.1 with 148); where it has two,
 // all, since what counts is the wider pair of them (64 x 28672 x 4096 gated 21.8 with 256, 21.4 with 296).
 static const int kUnit = 8;
-static int stream_width(int N, int shares) { return (N / kUnit + shares - 1) / shares * kUnit; }  // of the widest
+static int stream_width(int N, int shares) { return parts(N / kUnit, shares) * kUnit; }  // of the widest
 static int stream_shares(int N, bool gated, int at_once, int per) {
   const int units = N / kUnit, most = gated ? 16 : 32;
   const int rounds = (units + most * at_once - 1) / (most * at_once), all = rounds * at_once;
   const int shares = all < units / 2 ? all : units / 2;
-  return per == 1 ? (N + stream_width(N, shares) - 1) / stream_width(N, shares) : shares;
+  return per == 1 ? parts(N, stream_width(N, shares)) : shares;
 }
 static int stream_stages(int M, bool gated, int width, int s, int budget) {
   int stages = 12;  // (with 16 64 x 1024 x 8192 takes 7.3 us, not 7.0)
@@ -85,8 +83,9 @@ static double stream_cost(int M, int N, bool gated, int shares, int s, int at_on
 // through the same SM.  A tile takes no less than its outputs do, 3.1 and 1.9 us (gated 2.6: half
 // of the writers have none of a narrow tile).  Up front, and for the last tile's outputs: 5.6 and 3.9.  And
 // B has to be read.
-static double pair_cost(int tiles, bool gated, int cols, int K, double b_bytes, const DeviceInfo& di) {
-  const int pairs = di.sm_count / 2, rounds = (tiles + pairs - 1) / pairs;
+static double pair_cost(long long tiles, bool gated, int cols, int K, double b_bytes, const DeviceInfo& di) {
+  const int pairs = di.sm_count / 2;
+  const long long rounds = (tiles - 1) / pairs + 1;
   const double piece = split_sectors(K) ? (cols == 256 ? 0.42 : 0.32) : cols == 256 ? 0.30 : 0.195;
   const double products = igemm_kblocks(K) * piece, outputs = cols == 256 ? 3.1 : gated ? 2.6 : 1.9;
   const double start = cols == 256 ? 5.6 : 3.9, all = products + (rounds - 1) * (products > outputs ? products : outputs);
@@ -102,11 +101,11 @@ static void make_igemm_plan(int M, int N, int K, bool gated, b200q_igemm_plan_t*
   // (A last row tile of a few rows costs as much as any, but no more than that: 4097 x 12288 x 4096 takes 137.7 us, 4096 rows 132.5, and
   // 4096 rows with the last one in a kernel of its own beside them 142.2.)
   for (int cols = 256; cols >= 128; cols -= 128) {
-    const int tiles = pair_tiles(M, N, gated, cols);
+    const long long tiles = pair_tiles(M, N, gated, cols);
     const double cost = pair_cost(tiles, gated, cols, K, (double)(gated ? 2 : 1) * N * K, di);
     if (cost >= best) continue;
     best = cost;
-    *pl = {1, 256, cols, 2, cols == 256 ? 6 : 8, 2 * (tiles < di.sm_count / 2 ? tiles : di.sm_count / 2)};
+    *pl = {1, 256, cols, 2, cols == 256 ? 6 : 8, 2 * (int)(tiles < di.sm_count / 2 ? tiles : di.sm_count / 2)};
   }
   if (M > kStreamRows) return;
   const int* clusters = int8_stream_clusters(di);
@@ -201,10 +200,10 @@ static int run_igemm(const void* a, int lda, const void* b, int ldb, const float
     const CUresult r = enc(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, c, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return cuda_failed((int)r);
-    p.m_tiles = (int)(((long long)M + 255) / 256);
-    const int per = gated ? pc / 2 : pc;
-    p.n_tiles = (N + per - 1) / per;
-    if ((long long)p.m_tiles * p.n_tiles > 0x7fffffffll) return ST_UNSUPPORTED;
+    p.m_tiles = parts(M, 256);
+    p.n_tiles = parts(N, gated ? pc / 2 : pc);
+    // (more than any memory holds; a CTA's next tile stays an int)
+    if ((long long)p.m_tiles * p.n_tiles > 0x7fffff00ll) return ST_UNSUPPORTED;
     p.tiles = p.m_tiles * p.n_tiles;
     // rows of A that stay in the L2 cache while the columns of B stream past them: about 32 MB
     const long long fit = (32ll << 20) / (256ll * K);
@@ -242,7 +241,7 @@ static bool igemm_plan_ok(int M, int N, int K, bool gated, b200q_igemm_plan_t* p
   if (pl->width < kUnit || pl->width > (gated ? 128 : 256) || pl->width % kUnit != 0) return false;
   // (shares as the CTAs say, where these are of that width; else as few as there can be)
   int shares = pl->ctas > 0 && pl->ctas % pl->cluster == 0 ? pl->ctas / pl->cluster : 0;
-  if (shares < 1 || shares > N / kUnit || stream_width(N, shares) != pl->width) shares = (N + pl->width - 1) / pl->width;
+  if (shares < 1 || shares > N / kUnit || stream_width(N, shares) != pl->width) shares = parts(N, pl->width);
   pl->width = stream_width(N, shares);
   pl->ctas = shares * pl->cluster;
   return pl->stages >= 1 && pl->stages <= 16 &&
