@@ -1,8 +1,8 @@
-"""8-bit products at the ends of their range, against the definitions in 64 bits."""
+"""8-bit products and their sums at the ends of their range, against the definitions in 64 bits."""
 import pytest
 import torch
 
-from tests.test_gpu_int8 import _check, _exact
+from tests.test_gpu_int8 import F64, _check, _exact
 from tilus_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +38,28 @@ def test_nearly_2_to_the_31_rows():
     for p in places:
         want = _exact(a[p:p + 300], b, a_sf[p:p + 300], b_sf)
         _check(out[p:p + 300], want, torch.float16, 4 * 2.0 ** -24 * want.abs())
+
+
+@pytest.mark.parametrize("M,N", [(1, 16), (9, 64), (40, 512), (129, 1024), (260, 64), (700, 272)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_every_product_of_the_longest_sums_counts(M, N, gated):
+    """Partial sums of up to 2^30 that cancel to a small integer, which float16 holds: nothing is lost, nothing there twice.  (The
+    shapes go to each kernel, and to the stream kernel with and without a split of K.)"""
+    K, rows = 131056, 2 * N if gated else N
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    half = (K - 16) // 2
+    a = torch.full((M, K), -128, device="cuda", dtype=torch.int8)
+    b = torch.full((rows, K), 127, device="cuda", dtype=torch.int8)
+    b[:, :half] = -127
+    a[:, -16:] = torch.randint(-8, 8, (M, 16), generator=gen, device="cuda", dtype=torch.int8)
+    b[:, -16:] = torch.randint(-8, 8, (rows, 16), generator=gen, device="cuda", dtype=torch.int8)
+    sums = a[:, -16:].to(F64) @ b[:, -16:].to(F64).t()  # at most 16 * 8 * 8
+    one = torch.ones(M, device="cuda")
+    if gated:
+        got = ops.int8_gate_up(a, b, one, torch.full((rows,), 2.0 ** -8, device="cuda"))
+        g, u = (sums * 2.0 ** -8).chunk(2, dim=1)
+        want = g * torch.sigmoid(g) * u
+        _check(got, want, torch.float16, want.abs() * (14 + 1.2 * g.abs()) * 2.0 ** -23)
+    else:
+        got = ops.int8_matmul(a, b, one, torch.ones(rows, device="cuda"))
+        assert torch.equal(got.to(F64), sums)
