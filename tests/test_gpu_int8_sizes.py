@@ -1,8 +1,8 @@
-"""8-bit products and their sums at the ends of their range, against the definitions in 64 bits."""
+"""8-bit products, casts and their sums at the ends of their range, against the definitions in 64 bits."""
 import pytest
 import torch
 
-from tests.test_gpu_int8 import F64, _check, _exact
+from tests.test_gpu_int8 import F64, _cast_by_definition, _check, _exact
 from tilus_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -38,6 +38,18 @@ def test_nearly_2_to_the_31_rows():
     for p in places:
         want = _exact(a[p:p + 300], b, a_sf[p:p + 300], b_sf)
         _check(out[p:p + 300], want, torch.float16, 4 * 2.0 ** -24 * want.abs())
+
+
+def test_cast_of_nearly_2_to_the_31_rows():
+    T = 2 ** 31 - 1
+    x = torch.zeros(T, 8, device="cuda", dtype=torch.float16)
+    places = [0, T // 2 - 7, T - 50]
+    for p in places:
+        x[p:p + 50] = torch.randn(50, 8, device="cuda").half()
+    codes, sf = ops.per_token_cast_int8(x)
+    for p in places:
+        want, want_sf = _cast_by_definition(x[p:p + 50])
+        assert torch.equal(codes[p:p + 50], want) and torch.equal(sf[p:p + 50], want_sf)
 
 
 @pytest.mark.parametrize("M,N", [(1, 16), (9, 64), (40, 512), (129, 1024), (260, 64), (700, 272)])

@@ -952,7 +952,7 @@ static RowShape row_shape(int T, int D) {
   if (s.warp_rows) {
     s.vectors = nvec <= 32 ? 1 : nvec <= 64 ? 2 : nvec <= 128 ? 4 : 8;
     s.threads = 128;
-    s.ctas = (T + 3) / 4;
+    s.ctas = T / 4 + (T % 4 != 0);
     return s;
   }
   // (us, 256 threads / 512: 4096 x 8192 53.2 / 48.3, with a 32-bit residual 69.0 / 61.7; 4096 x 6144 44.6 / 48.3, 55.0 / 61.5; 2048 x 16384
@@ -1050,7 +1050,7 @@ void norm_backward_shape(int D, bool residual_f32, int gates, int tokens_per_gat
   const int per_sm = NORM_BACK_THREADS / p->threads < 8 ? NORM_BACK_THREADS / p->threads : 8, most = sms * per_sm;
   // Runs that a gate's rows are enough for: a row each where the SMs are as many, else two, since a CTA's sums over rows are as many bytes
   // as six rows.  (us, two rows each / one: 8 x 4096 9.3 / 7.9, 148 x 4096 10.3 / 8.9, 296 x 1024 7.4 / 7.7.)
-  const int single = sms / gates < tokens_per_gate ? sms / gates : tokens_per_gate, twos = (tokens_per_gate + 1) / 2;
+  const int single = sms / gates < tokens_per_gate ? sms / gates : tokens_per_gate, twos = tokens_per_gate / 2 + tokens_per_gate % 2;
   const int runs = single > twos ? single : twos;
   if (gates >= most) {
     p->ctas_per_gate = 1;
