@@ -18,8 +18,8 @@
 //   stream  up to 256 rows, all of them against an equal share of the columns in each CTA, so that B is read once: bound by that.
 //   row     up to 16 rows where the product is small: no pipeline to fill, mma.sync from registers.  Bound by the latency of its loads.
 // On a B200, in a graph of such calls: pair, 4096 x 8192 x 8192, 162 us (3.40 POP/s, the tensor pipe busy 88 % of the time); 4096 x 28672
-// x 8192 gated 558 to 642 us as the power limit has it (3.0 to 3.4 POP/s); stream, 8 x 28672 x 4096 gated 20.5 us (5.7 TB/s), 1 x 16384 x
-// 8192 23.6 us (5.7 TB/s), 64 x 28672 x 4096 gated 21.4 us; row, 1 x 4096 x 4096 3.6 us.
+// x 8192 gated 541 to 642 us as the power limit has it (3.0 to 3.5 POP/s); stream, 8 x 28672 x 4096 gated 20.5 us (5.7 TB/s; 23.4 on
+// GPUs that read slower), 64 x 28672 x 4096 gated 21.6 us; row, 1 x 4096 x 4096 5.0 us, 3.9 with B read early.
 //
 // All are launched with programmatic stream serialization: they set up under the end of the kernel before them.  All they read
 // before that kernel has ended is, in the stream and row kernels and where the caller says that it may (`early`), rows of B; the
@@ -664,8 +664,9 @@ __global__ void __launch_bounds__(S_THREADS)
 // reads its part of B straight from memory into the registers that mma.sync takes it from: 16 consecutive bytes of a row are the
 // four words of two steps, since the order of K inside a sum is free as long as A's words go by the same order.  Nothing passes
 // through shared memory but the warps' sums, and there is no pipeline to fill: what a small product takes is little more than the
-// latency of its loads.  (M = 1, us, the stream kernel / this one: 4096 x 4096 6.7 / 4.1, 1024 x 4096 4.5 / 2.3; with 16 rows, whose
-// loads are as many as B's, 8192 x 8192 14.5 / 18.5.)
+// latency of its loads.  (us, the stream kernel / this one: 1 x 4096 x 4096 8.1 / 5.1, 4 x 1024 x 4096 5.6 / 3.5; with 12 rows, whose
+// loads are as many as B's, 1504 x 11008 8.2 / 10.2.  B read early takes 0.3 to 1.1 us off this one: its loads are what it consists of.
+// Rows on their way to L2 instead gave nothing that held over sizes: 1 x 4096 x 4096 4.5 for 5.1, 8 x 14336 x 4096 15.9 for 15.2.)
 constexpr int R_WARPS = 16;
 constexpr int R_BATCH = 4;  // 64-byte pieces of two rows that a thread has in flight
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -955,8 +955,9 @@ static RowShape row_shape(int T, int D) {
     s.ctas = T / 4 + (T % 4 != 0);
     return s;
   }
-  // (us, 256 threads / 512: 4096 x 8192 53.2 / 48.3, with a 32-bit residual 69.0 / 61.7; 4096 x 6144 44.6 / 48.3, 55.0 / 61.5; 2048 x 16384
-  // 54.4 / 69.8)
+  // (us for 4096 rows, 256 threads / 512.  32-bit residual: 5120 channels 42.3 / 39.1, 6144 54.1 / 48.4, 7168 59.3 / 54.3, 8192 65.4 / 61.0,
+  // 8200 82.0 / 92.0.  16-bit: 33.5 / 38.3 for 6144, 38.8 / 42.0 for 7168, 43.5 / 45.6 for 8192, 51.0 / 46.0 for 8200.  So the band is right
+  // for 32-bit residuals, could begin lower there, and costs 16-bit ones up to a tenth.)
   const int threads = T <= 296 || (nvec > 768 && nvec <= 1024) ? 512 : 256;
   s.vectors = 1;
   while (s.vectors < 8 && s.vectors * threads < nvec) s.vectors *= 2;
