@@ -195,8 +195,8 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_sf: torch.Tensor, b_sf: torc
     this call; ``out`` is a tensor without a gradient.
 
     ``early_b``: ``b`` may be read while the stream's previous kernel still runs.  Say so only where ``b`` was complete
-    before that kernel started: weights at rest, with a cast, norm or product of this library between what wrote them (on any
-    stream) and this call.  It saves a small product up to 1 us."""
+    before that kernel started: weights at rest, with an int8 cast, a block norm or an 8-bit product on this stream between
+    what wrote them (on any stream) and this call.  It saves a small product up to 1 us."""
     return _lib.native().igemm(a, b, a_sf, b_sf, bias, act_code(out_dtype), False, None, out, early_b)
 
 
